@@ -4,6 +4,6 @@ Importing the package loads the CUDA library and raises ImportError when it has 
 computes attention on the CPU.
 """
 from . import _lib
-from .api import (KV_F16, KV_NAMES, KV_Q4, KV_Q4K4, KV_Q8, Context, RqCudaError, Sequence, device_count)  # noqa: F401
+from .api import (KV_F16, KV_NAMES, KV_Q4, KV_Q4K4, KV_Q8, Context, Q4Matrix, RqCudaError, Sequence, device_count)  # noqa: F401
 
 _lib.load()

@@ -95,6 +95,13 @@ PROTOTYPES = {
     "rq_cuda_dn_set_weights": (_i, [_vp, _i, _vp, _vp, _vp, _vp]),
     "rq_cuda_dn_prep_dev": (_i, [_vp, _i, _vp]),
     "rq_cuda_dn_out_dev": (_i, [_vp, _i, _vp, _vp]),
+    "rq_cuda_q4_new": (_i, [_vp, _i, _i, _i, _vp, _vp, _pp]),
+    "rq_cuda_q4_new_dev": (_i, [_vp, _i, _i, _i, _vp, _vp, _pp]),
+    "rq_cuda_q4_free": (None, [_vp]),
+    "rq_cuda_q4_bytes": (_sz, [_vp]),
+    "rq_cuda_add_norm_quant_dev": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp]),
+    "rq_cuda_mm_q4_dev": (_i, [_vp, _vp, _i, _vp, _vp, _vp]),
+    "rq_cuda_ffn_q4_dev": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "rq_cuda_malloc": (_i, [_vp, _sz, _pp]),
     "rq_cuda_mfree": (_i, [_vp, _vp]),
     "rq_cuda_malloc_host": (_i, [_vp, _sz, _pp]),

@@ -5,6 +5,7 @@ DeltaNet state (RqSeq), and passes over segments of rows (rq_forward_batch; refe
 call per layer.  All arithmetic happens inside librq_cuda.so; numpy arrays are only the host buffers.
 """
 import ctypes as C
+import weakref
 
 import numpy as np
 
@@ -53,6 +54,7 @@ class Context:
         self.vdim = dn_nv * dn_dv
         self.nrows = 0
         self._seqs = []
+        self._q4s = weakref.WeakSet()
 
     # -- errors
     def check(self, rc):
@@ -63,6 +65,8 @@ class Context:
         if self.h:
             for s in list(self._seqs):
                 s.free()
+            for m in list(self._q4s):
+                m.free()
             self.L.rq_cuda_free(self.h)
             self.h = None
 
@@ -211,6 +215,32 @@ class Context:
 
     def dn_rec_dev(self, lin_layer, rows_dev, out_dev):
         self.check(self.L.rq_cuda_dn_rec_dev(self.h, lin_layer, _ptr(rows_dev), _ptr(out_dev)))
+
+    # -- the products around the attention (device pointers as ints, None for NULL)
+    def q4_new(self, levels, scales, gs):
+        """A 4-bit weight matrix from host arrays: levels [n][k / 2] uint8 (two levels + 8 in a byte), scales [n][k / gs] float16."""
+        levels = np.ascontiguousarray(levels, np.uint8)
+        scales = np.ascontiguousarray(scales, np.float16)
+        n, k = levels.shape[0], levels.shape[1] * 2
+        if gs < 1 or k % gs or scales.shape != (n, k // gs):
+            raise ValueError("levels must be [n][k / 2] and scales [n][k / gs]")
+        return Q4Matrix(self, self.L.rq_cuda_q4_new, n, k, gs, _ptr(levels), _ptr(scales))
+
+    def q4_new_dev(self, n, k, gs, levels_dev, scales_dev):
+        """The same from device memory."""
+        return Q4Matrix(self, self.L.rq_cuda_q4_new_dev, n, k, gs, levels_dev, scales_dev)
+
+    def add_norm_quant_dev(self, rows, dim, gs, x_dev, delta_dev, w_dev, eps, x_out_dev, y_dev, xq_dev, xs_dev):
+        """x + delta -> x_out; RMS norm with weights w -> y (fp32) and / or xq, xs (int8 levels, scales per gs values)."""
+        self.check(self.L.rq_cuda_add_norm_quant_dev(self.h, rows, dim, gs, x_dev, delta_dev, w_dev, eps, x_out_dev, y_dev, xq_dev, xs_dev))
+
+    def mm_q4_dev(self, w, rows, xq_dev, xs_dev, out_dev):
+        """out [rows][n] = the 8-bit rows times the 4-bit matrix w."""
+        self.check(self.L.rq_cuda_mm_q4_dev(self.h, w.h, rows, xq_dev, xs_dev, out_dev))
+
+    def ffn_q4_dev(self, gate, up, rows, xq_dev, xs_dev, h_dev, hq_dev, hs_dev):
+        """h = silu(x gate^T) (x up^T) as fp32 rows (h_dev) and / or 8-bit rows (hq_dev, hs_dev)."""
+        self.check(self.L.rq_cuda_ffn_q4_dev(self.h, gate.h, up.h, rows, xq_dev, xs_dev, h_dev, hq_dev, hs_dev))
 
     # -- convenience: one whole pass
     def attention(self, layer, segments, q, k=None, v=None, prefill=False, commit=True):
@@ -365,3 +395,31 @@ class Sequence:
         st = np.ascontiguousarray(st, np.float32)
         assert st.size == self.state_floats()
         self.ctx.check(self.ctx.L.rq_cuda_seq_write_state(self.h, lin_layer, _ptr(st)))
+
+
+class Q4Matrix:
+    """A 4-bit weight matrix laid out in device memory; freed with the object (or with its context)."""
+
+    def __init__(self, ctx, make, n, k, gs, levels, scales):
+        self.h = None
+        self.ctx = ctx
+        h = C.c_void_p()
+        ctx.check(make(ctx.h, n, k, gs, levels, scales, C.byref(h)))
+        self.h = h
+        self.n, self.k, self.gs = n, k, gs
+        ctx._q4s.add(self)
+
+    def free(self):
+        if self.h and self.ctx.h:
+            self.ctx.L.rq_cuda_q4_free(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    @property
+    def nbytes(self):
+        return self.ctx.L.rq_cuda_q4_bytes(self.h)

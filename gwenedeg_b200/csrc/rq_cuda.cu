@@ -26,6 +26,8 @@
 #include "deltanet_chunk.cuh"
 #include "kv_dequant.cuh"
 #include "kv_store.cuh"
+#include "norm_quant.cuh"
+#include "q4_mm.cuh"
 
 using namespace rq;
 
@@ -1792,6 +1794,158 @@ int rq_cuda_dn_out_dev(RqCuda *c, int lin_layer, const float *rows, float *out) 
     dn_out_kernel<<<dim3(c->nrows, m.dn_nv), 128, 0, c->stream>>>(m.dn_nk, m.dn_nv, norm, rows, lw, out);
     c->launches++;
     CU(c, cudaGetLastError());
+    return RQ_CUDA_OK;
+}
+
+// ---------------------------------------------------------------------------------------------------- the products around it
+}  // extern "C"
+
+struct RqCudaQ4 {
+    RqCuda *ctx;
+    Q4View v;
+    uint8_t *mem;  // levels, then scales
+    size_t bytes;
+};
+
+static bool q4_gs_ok(int gs) { return gs == 32 || gs == 64 || gs == 128; }
+
+// a matrix of the given shape with its device memory, contents unset
+static int q4_alloc(RqCuda *c, int n, int k, int gs, const void *levels, const void *scales, RqCudaQ4 **out) {
+    if (!c || !out) return RQ_CUDA_ERR_ARG;
+    *out = nullptr;
+    if (!levels || !scales) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: null argument");
+    if (n < 1 || n > (1 << 30) || k < 1 || k > (1 << 30) || !q4_gs_ok(gs) || k % gs) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: %d x %d in groups of %d", n, k, gs);
+    CU(c, cudaSetDevice(c->device));
+    RqCudaQ4 *w = new (std::nothrow) RqCudaQ4();
+    if (!w) return fail(c, RQ_CUDA_ERR_NOMEM, "host allocation");
+    Q4View &v = w->v;
+    v.n = n, v.k = k, v.gs = gs;
+    v.tiles = (n + Q4_TILE - 1) / Q4_TILE;
+    v.chunks = (k + Q4_CHUNK - 1) / Q4_CHUNK;
+    v.slices = (k + Q4_SLICE - 1) / Q4_SLICE;
+    const size_t lb = (size_t)v.tiles * v.chunks * 1024, sb = (size_t)v.tiles * v.slices * Q4_TILE * (Q4_SLICE / gs) * 2;
+    w->ctx = c;
+    w->bytes = lb + sb;
+    const cudaError_t e = cudaMalloc((void **)&w->mem, w->bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        delete w;
+        return fail(c, RQ_CUDA_ERR_NOMEM, "4-bit matrix of %zu bytes: %s", lb + sb, cudaGetErrorString(e));
+    }
+    v.levels = (const uint4 *)w->mem;
+    v.scales = (const __half *)(w->mem + lb);
+    *out = w;
+    return RQ_CUDA_OK;
+}
+
+// lays the matrix out from device memory and waits for it
+static int q4_fill(RqCuda *c, RqCudaQ4 *w, const uint8_t *levels, const void *scales) {
+    CU(c, launch_q4_pack(levels, (const __half *)scales, w->v, c->stream));
+    c->launches += 2;
+    CU(c, cudaStreamSynchronize(c->stream));
+    return RQ_CUDA_OK;
+}
+
+extern "C" {
+
+void rq_cuda_q4_free(RqCudaQ4 *w) {
+    if (!w) return;
+    cudaSetDevice(w->ctx->device);
+    cudaStreamSynchronize(w->ctx->stream);
+    cudaFree(w->mem);
+    delete w;
+}
+
+size_t rq_cuda_q4_bytes(const RqCudaQ4 *w) { return w ? w->bytes : 0; }
+
+int rq_cuda_q4_new_dev(RqCuda *c, int n, int k, int gs, const unsigned char *levels, const unsigned short *scales, RqCudaQ4 **out) {
+    if (c && levels && scales && (((uintptr_t)levels & 3) || ((uintptr_t)scales & 1))) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: levels must be 4-byte, scales 2-byte aligned");
+    int rc = q4_alloc(c, n, k, gs, levels, scales, out);
+    if (rc) return rc;
+    if ((rc = q4_fill(c, *out, levels, scales))) {
+        rq_cuda_q4_free(*out);
+        *out = nullptr;
+    }
+    return rc;
+}
+
+int rq_cuda_q4_new(RqCuda *c, int n, int k, int gs, const unsigned char *levels, const unsigned short *scales, RqCudaQ4 **out) {
+    int rc = q4_alloc(c, n, k, gs, levels, scales, out);
+    if (rc) return rc;
+    const size_t lb = ((size_t)n * (k / 2) + 15) & ~(size_t)15, sb = (size_t)n * (k / gs) * 2;
+    uint8_t *tmp = nullptr;
+    cudaError_t e = cudaMalloc((void **)&tmp, lb + sb);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(tmp, levels, (size_t)n * (k / 2), cudaMemcpyHostToDevice, c->stream);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(tmp + lb, scales, sb, cudaMemcpyHostToDevice, c->stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        rc = fail(c, e == cudaErrorMemoryAllocation ? RQ_CUDA_ERR_NOMEM : RQ_CUDA_ERR_DEVICE, "q4_new: %s", cudaGetErrorString(e));
+    } else {
+        rc = q4_fill(c, *out, tmp, tmp + lb);
+    }
+    if (tmp) {
+        cudaStreamSynchronize(c->stream);
+        cudaFree(tmp);
+    }
+    if (rc) {
+        rq_cuda_q4_free(*out);
+        *out = nullptr;
+    }
+    return rc;
+}
+
+int rq_cuda_add_norm_quant_dev(RqCuda *c, int rows, int dim, int gs, const float *x, const float *delta, const float *w, float eps, float *x_out,
+                               float *y, signed char *xq, float *xs) {
+    if (!c) return RQ_CUDA_ERR_ARG;
+    if (!x || !w || !xq != !xs || (!y && !xq && !x_out)) return fail(c, RQ_CUDA_ERR_ARG, "add_norm_quant: null argument");
+    if (rows < 1 || rows > c->max_rows) return fail(c, RQ_CUDA_ERR_ARG, "add_norm_quant: %d rows (at most %d)", rows, c->max_rows);
+    if (!q4_gs_ok(gs) || dim < gs || dim % gs || dim > NORM_MAX_DIM) return fail(c, RQ_CUDA_ERR_ARG, "add_norm_quant: rows of %d in groups of %d", dim, gs);
+    if (!(eps >= 0.0f)) return fail(c, RQ_CUDA_ERR_ARG, "add_norm_quant: eps %g", (double)eps);
+    NEED_ALIGNED(c, "add_norm_quant", x, delta, w, x_out, y);
+    if (((uintptr_t)xq & 3) || ((uintptr_t)xs & 3)) return fail(c, RQ_CUDA_ERR_ARG, "add_norm_quant: xq and xs must be 4-byte aligned");
+    CU(c, cudaSetDevice(c->device));
+    const NormQuantArgs a = {x, delta, w, x_out, y, (int8_t *)xq, xs, dim, eps};
+    CU(c, launch_add_norm_quant(a, rows, gs, c->stream));
+    c->launches++;
+    return RQ_CUDA_OK;
+}
+
+static int q4_check(RqCuda *c, const char *what, const RqCudaQ4 *w, int rows, const void *xq, const void *xs) {
+    if (!w || !xq || !xs) return fail(c, RQ_CUDA_ERR_ARG, "%s: null argument", what);
+    if (w->ctx != c) return fail(c, RQ_CUDA_ERR_ARG, "%s: the matrix belongs to another context", what);
+    if (rows < 1 || rows > c->max_rows) return fail(c, RQ_CUDA_ERR_ARG, "%s: %d rows (at most %d)", what, rows, c->max_rows);
+    NEED_ALIGNED(c, what, xq);
+    if ((uintptr_t)xs & 3) return fail(c, RQ_CUDA_ERR_ARG, "%s: xs must be 4-byte aligned", what);
+    return RQ_CUDA_OK;
+}
+
+int rq_cuda_mm_q4_dev(RqCuda *c, const RqCudaQ4 *w, int rows, const signed char *xq, const float *xs, float *out) {
+    if (!c) return RQ_CUDA_ERR_ARG;
+    int rc = q4_check(c, "mm_q4", w, rows, xq, xs);
+    if (rc) return rc;
+    if (!out || ((uintptr_t)out & 3)) return fail(c, RQ_CUDA_ERR_ARG, "mm_q4: out is null or not 4-byte aligned");
+    CU(c, cudaSetDevice(c->device));
+    const Q4Args a = {w->v, w->v, (const int8_t *)xq, xs, rows, out, nullptr, nullptr};
+    CU(c, launch_q4(a, false, c->stream));
+    c->launches++;
+    return RQ_CUDA_OK;
+}
+
+int rq_cuda_ffn_q4_dev(RqCuda *c, const RqCudaQ4 *gate, const RqCudaQ4 *up, int rows, const signed char *xq, const float *xs, float *h,
+                       signed char *hq, float *hs) {
+    if (!c) return RQ_CUDA_ERR_ARG;
+    int rc = q4_check(c, "ffn_q4", gate, rows, xq, xs);
+    if (!rc) rc = q4_check(c, "ffn_q4", up, rows, xq, xs);
+    if (rc) return rc;
+    const Q4View &g = gate->v, &u = up->v;
+    if (g.n != u.n || g.k != u.k || g.gs != u.gs) return fail(c, RQ_CUDA_ERR_ARG, "ffn_q4: matrices %d x %d / %d and %d x %d / %d", g.n, g.k, g.gs, u.n, u.k, u.gs);
+    if (!hq != !hs || (!h && !hq)) return fail(c, RQ_CUDA_ERR_ARG, "ffn_q4: null argument");
+    if (((uintptr_t)h & 3) || ((uintptr_t)hs & 3)) return fail(c, RQ_CUDA_ERR_ARG, "ffn_q4: h and hs must be 4-byte aligned");
+    if (hq && g.n % g.gs) return fail(c, RQ_CUDA_ERR_ARG, "ffn_q4: %d outputs do not fill groups of %d", g.n, g.gs);
+    CU(c, cudaSetDevice(c->device));
+    const Q4Args a = {g, u, (const int8_t *)xq, xs, rows, h, (int8_t *)hq, hs};
+    CU(c, launch_q4(a, true, c->stream));
+    c->launches++;
     return RQ_CUDA_OK;
 }
 

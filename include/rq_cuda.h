@@ -307,6 +307,44 @@ int rq_cuda_dn_set_weights(RqCuda *ctx, int lin_layer, const float *conv, const 
 int rq_cuda_dn_prep_dev(RqCuda *ctx, int lin_layer, float *rows_dev);
 int rq_cuda_dn_out_dev(RqCuda *ctx, int lin_layer, const float *rows_dev, float *out_dev);
 
+/* ---- the products around the attention (device pointers) ---------------------------------------------------- */
+/* What the reference's workers do between two attention calls, for hosts that keep their activations on the device: the
+ * residual addition + norm + quantiser (rmsnorm, forward.c:886; quantize, :803), the matrix products with quantised weights
+ * (rows_mm, :3315) and the gated feed-forward product (swiglu, :1953).  Rows travel in 8 bits: int8 levels [rows][k] and one
+ * fp32 scale per gs values [rows][k / gs], as rq_cuda_set_wo_quant and the calls below leave them; weights have 4 bits.  A
+ * decode layer is: rq_cuda_add_norm_quant_dev, rq_cuda_mm_q4_dev (q, k, v), rq_cuda_qk_norm_rope_store_dev, the attention
+ * with rq_cuda_set_wo_quant, rq_cuda_mm_q4_dev (wo), rq_cuda_add_norm_quant_dev, rq_cuda_ffn_q4_dev, rq_cuda_mm_q4_dev (down).
+ * These calls need no open pass; 1 <= rows <= max_rows.  They allocate nothing, use no scratch of the context and can be
+ * captured into CUDA graphs.  Outputs must not overlap inputs except where a call says so.
+ *
+ * A 4-bit weight matrix of n outputs x k inputs, laid out on the device once (RqCudaQ4).  levels: [n][k / 2] bytes, input 2 j
+ * in the low half of byte j, input 2 j + 1 in the high half, each the level (-8 .. 7) + 8; scales: [n][k / gs] IEEE half bits;
+ * weight = level x scale.  gs: 32, 64 or 128, dividing k.  _new takes host pointers, _new_dev device pointers (both return when the
+ * matrix is complete; the sources may then be freed).  Matrices are freed before their context. */
+typedef struct RqCudaQ4 RqCudaQ4;
+int rq_cuda_q4_new(RqCuda *ctx, int n, int k, int gs, const unsigned char *levels, const unsigned short *scales, RqCudaQ4 **w);
+int rq_cuda_q4_new_dev(RqCuda *ctx, int n, int k, int gs, const unsigned char *levels_dev, const unsigned short *scales_dev, RqCudaQ4 **w);
+void rq_cuda_q4_free(RqCudaQ4 *w);
+size_t rq_cuda_q4_bytes(const RqCudaQ4 *w); /* device memory it holds */
+/* x' = x + delta per element (delta NULL: x' = x), written to x_out (may be x itself; NULL: not written); then per row
+ * inv = 1 / sqrt(mean(x'^2) + eps) and v = w x'; y = v inv (NULL: not written); xq, xs (both NULL: not written): per group of gs
+ * values the levels of the library's quantiser (rq_cuda_set_wo_quant) on v and scale = max|v| (1 / 127) inv.  inv cancels out
+ * of the levels: they are a function of x', w and the group alone.  dim: a multiple of gs, at most 32768; gs 32, 64 or 128.
+ * x, x_out, delta, w, y 16-byte aligned; xq, xs 4-byte aligned. */
+int rq_cuda_add_norm_quant_dev(RqCuda *ctx, int rows, int dim, int gs, const float *x_dev, const float *delta_dev, const float *w_dev,
+                               float eps, float *x_out_dev, float *y_dev, signed char *xq_dev, float *xs_dev);
+/* out[r][f] = sum over groups of xs[r][g] scale[f][g] (sum over the group of xq[r][k] level[f][k]): rows xq [rows][k], xs
+ * [rows][k / gs] times the matrix, out fp32 [rows][n].  The inner sum is an exact integer; the outer one is in fp32 in one fixed
+ * order (chains of fused multiply-adds inside slices of 512 inputs, slices added in order), so that a row's result does not
+ * depend on the other rows of the call.  xq 16-byte aligned, xs and out 4-byte aligned. */
+int rq_cuda_mm_q4_dev(RqCuda *ctx, const RqCudaQ4 *w, int rows, const signed char *xq_dev, const float *xs_dev, float *out_dev);
+/* The gated feed-forward product in one kernel: h = silu(x gate^T) (x up^T), silu(g) = g / (1 + e^-g), both products as
+ * rq_cuda_mm_q4_dev.  h_dev: fp32 [rows][n]; hq_dev, hs_dev: the same rows through the library's quantiser, levels [rows][n] and
+ * scales [rows][n / gs] with the matrices' gs (n a multiple of gs then), ready for the down product.  Either h_dev or the pair
+ * may be NULL.  gate and up have the same shape and gs; both may be the same matrix. */
+int rq_cuda_ffn_q4_dev(RqCuda *ctx, const RqCudaQ4 *gate, const RqCudaQ4 *up, int rows, const signed char *xq_dev, const float *xs_dev,
+                       float *h_dev, signed char *hq_dev, float *hs_dev);
+
 /* ---- device memory and timing helpers for hosts without a CUDA runtime of their own (ctypes, cgo, JNI) ---- */
 int rq_cuda_malloc(RqCuda *ctx, size_t bytes, void **dev);
 int rq_cuda_mfree(RqCuda *ctx, void *dev);
