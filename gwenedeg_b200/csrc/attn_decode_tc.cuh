@@ -87,17 +87,6 @@ cudaError_t launch_attn_part_tc(const AttnPartTcArgs &a, cudaStream_t stream);
 
 #ifdef RQ_ATTN_DECODE_TC_INSTANTIATE
 
-// instruction descriptor of tcgen05.mma kind::i8: int8 / uint8 operands, int32 accumulator, M x N; a_mn / b_mn: MN-major (1) or
-// K-major (0); a_s / b_s: signed (1) or unsigned (0) 8-bit values
-__host__ __device__ constexpr uint32_t umma_idesc_i8(int M, int N, int a_mn, int b_mn, int a_s, int b_s) {
-    return (2u << 4) | ((uint32_t)a_s << 7) | ((uint32_t)b_s << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) |
-           ((uint32_t)(M >> 4) << 24);
-}
-__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem), "l"(a), "l"(b),
-                 "r"(idesc), "r"(acc)
-                 : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *m, int x, int y, int z, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
                      smem_u32(dst)),
@@ -178,21 +167,6 @@ __device__ __forceinline__ int f32_ord(float f) {
     return b >= 0 ? b : b ^ 0x7fffffff;
 }
 __device__ __forceinline__ float ord_f32(int b) { return __int_as_float(b >= 0 ? b : b ^ 0x7fffffff); }
-
-// One CTA's teardown wait for a copy that may still be in flight once a wait has expired: polls for at most ~2 ms whatever
-// the status word says, so that the CTA does not leave while a copy still writes its shared memory.
-__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity) {
-    unsigned long long t0 = 0;
-    for (int it = 0; it < (1 << 22); it++) {
-        if (mbar_try_wait(bar, parity)) return;
-        if ((it & 255) == 255) {
-            unsigned long long now;
-            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-            if (t0 == 0) t0 = now;
-            if (now - t0 > 2000000ull) return;
-        }
-    }
-}
 
 // Persistent form: the grid is two CTAs per SM (one for 5..8 vectors per KV head), each CTA walks a contiguous range of the work
 // items (KV head g, block gb of the pass) in the order j = g total_blocks + gb, so that consecutive items mostly share their row

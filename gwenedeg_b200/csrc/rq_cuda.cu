@@ -1814,7 +1814,7 @@ static int q4_alloc(RqCuda *c, int n, int k, int gs, const void *levels, const v
     if (!c || !out) return RQ_CUDA_ERR_ARG;
     *out = nullptr;
     if (!levels || !scales) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: null argument");
-    if (n < 1 || n > (1 << 30) || k < 1 || k > (1 << 30) || !q4_gs_ok(gs) || k % gs) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: %d x %d in groups of %d", n, k, gs);
+    if (n < 1 || n > (1 << 21) || k < 1 || k > (1 << 30) || !q4_gs_ok(gs) || k % gs) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: %d x %d in groups of %d", n, k, gs);
     CU(c, cudaSetDevice(c->device));
     RqCudaQ4 *w = new (std::nothrow) RqCudaQ4();
     if (!w) return fail(c, RQ_CUDA_ERR_NOMEM, "host allocation");
@@ -1926,7 +1926,7 @@ int rq_cuda_mm_q4_dev(RqCuda *c, const RqCudaQ4 *w, int rows, const signed char 
     if (!out || ((uintptr_t)out & 3)) return fail(c, RQ_CUDA_ERR_ARG, "mm_q4: out is null or not 4-byte aligned");
     CU(c, cudaSetDevice(c->device));
     const Q4Args a = {w->v, w->v, (const int8_t *)xq, xs, rows, out, nullptr, nullptr};
-    CU(c, launch_q4(a, false, c->stream));
+    CU(c, launch_q4(a, false, c->n_sm, tm_encode(), c->d_err, c->stream));
     c->launches++;
     return RQ_CUDA_OK;
 }
@@ -1944,7 +1944,7 @@ int rq_cuda_ffn_q4_dev(RqCuda *c, const RqCudaQ4 *gate, const RqCudaQ4 *up, int 
     if (hq && g.n % g.gs) return fail(c, RQ_CUDA_ERR_ARG, "ffn_q4: %d outputs do not fill groups of %d", g.n, g.gs);
     CU(c, cudaSetDevice(c->device));
     const Q4Args a = {g, u, (const int8_t *)xq, xs, rows, h, (int8_t *)hq, hs};
-    CU(c, launch_q4(a, true, c->stream));
+    CU(c, launch_q4(a, true, c->n_sm, tm_encode(), c->d_err, c->stream));
     c->launches++;
     return RQ_CUDA_OK;
 }

@@ -335,7 +335,7 @@ int rq_cuda_add_norm_quant_dev(RqCuda *ctx, int rows, int dim, int gs, const flo
                                float eps, float *x_out_dev, float *y_dev, signed char *xq_dev, float *xs_dev);
 /* out[r][f] = sum over groups of xs[r][g] scale[f][g] (sum over the group of xq[r][k] level[f][k]): rows xq [rows][k], xs
  * [rows][k / gs] times the matrix, out fp32 [rows][n].  The inner sum is an exact integer; the outer one is in fp32 in one fixed
- * order (chains of fused multiply-adds inside slices of 512 inputs, slices added in order), so that a row's result does not
+ * order (chains of fused multiply-adds inside slices of 512 inputs, slices added in pairs, pairs in order), so that a row's result does not
  * depend on the other rows of the call.  xq 16-byte aligned, xs and out 4-byte aligned. */
 int rq_cuda_mm_q4_dev(RqCuda *ctx, const RqCudaQ4 *w, int rows, const signed char *xq_dev, const float *xs_dev, float *out_dev);
 /* The gated feed-forward product in one kernel: h = silu(x gate^T) (x up^T), silu(g) = g / (1 + e^-g), both products as
