@@ -93,12 +93,6 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *m, int
                  "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                  : "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr));
-}
-
 // The query vectors of one (row, KV head), once per pass and layer: rotated as att_q_rot does (reference src/forward.c:1662:
 // signs, butterflies h = 1, 2, 4, ..., scaling by 1 / head_dim) in fp32, then per (vector v, 32-dim group c) 16-bit fixed point
 // q = qs[v][c] (256 hi + lo), hi and lo in [-128, 127], laid out as the B operand of the score MMAs: rows 2 v (hi) and 2 v + 1

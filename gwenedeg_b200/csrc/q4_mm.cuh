@@ -4,7 +4,7 @@
 //
 // xq, xs: the rows as the quantisers of this library leave them (int8 levels, one fp32 scale per group); wq: levels -8 .. 7, ws: f16.
 // The sum over groups has one order, whatever kernel runs and however many rows a pass has: inputs are cut into slices of 512, a
-// slice's groups are a chain p = fma(D, ws xs, p) in ascending order from 0, two adjacent slices are added (the last one may be alone),
+// slice's groups are a chain p = fma(round(D ws), xs, p) in ascending order from 0, two adjacent slices are added (the last one may be alone),
 // and the pairs are added in ascending order from 0.
 // So a row's result does not depend on the other rows of the pass.
 #pragma once
@@ -95,8 +95,10 @@ __device__ __forceinline__ void mma_s8(int *d, const uint32_t *a, uint32_t b0, u
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// An int32 accumulator that starts at the bits of 1.5 2^23 ends as the bits of the float 1.5 2^23 + sum, exactly, while |sum| < 2^22
-// (here |16 D| <= 16 . 128 . 8 . 128 = 2^21): one subtraction instead of an integer conversion.
+// An int32 sum S plus the bits of 1.5 2^23 are the bits of the float 1.5 2^23 + S, exactly, while |S| < 2^22 (here S = 16 D, as the levels
+// sit in the upper halves of their bytes: |S| <= 16 . 128 . 8 . 128 = 2^21).  With v = ws / 16, M = 1.5 2^23:  fma(M + S, v, -M v) =
+// round(D ws): M v is exact (ws has 11 significant bits), so one multiply-add converts, removes the offset and applies the weight's
+// scale, with the one rounding of the product.
 constexpr int Q4_MAGIC = 0x4B400000;
 constexpr float Q4_MAGIC_F = 12582912.0f;
 
@@ -184,7 +186,6 @@ __global__ void __launch_bounds__(256) q4_rows_kernel(const Q4Args a) {
                                     A[m][st][2] = lo & 0xF0F0F0F0u;
                                     A[m][st][3] = hi & 0xF0F0F0F0u;
                                 }
-                                // (1 / 16: the levels are in the upper halves of their bytes)
                                 ws[m][0] = __half2float(ss[m][c * GC + gc]) * 0.0625f;
                                 ws[m][1] = __half2float(ss[m][8 * PER + c * GC + gc]) * 0.0625f;
                             }
@@ -204,10 +205,11 @@ __global__ void __launch_bounds__(256) q4_rows_kernel(const Q4Args a) {
                                     const float x0 = __ldg(xs + (size_t)min(8 * j + 2 * t, rows - 1) * G), x1 = __ldg(xs + (size_t)min(8 * j + 2 * t + 1, rows - 1) * G);
 #pragma unroll
                                     for (int m = 0; m < MT; m++) {
-                                        p[m][j][0] = fmaf(__int_as_float(d[m][0]) - Q4_MAGIC_F, ws[m][0] * x0, p[m][j][0]);
-                                        p[m][j][1] = fmaf(__int_as_float(d[m][1]) - Q4_MAGIC_F, ws[m][0] * x1, p[m][j][1]);
-                                        p[m][j][2] = fmaf(__int_as_float(d[m][2]) - Q4_MAGIC_F, ws[m][1] * x0, p[m][j][2]);
-                                        p[m][j][3] = fmaf(__int_as_float(d[m][3]) - Q4_MAGIC_F, ws[m][1] * x1, p[m][j][3]);
+                                        const float o0 = -Q4_MAGIC_F * ws[m][0], o1 = -Q4_MAGIC_F * ws[m][1];
+                                        p[m][j][0] = fmaf(fmaf(__int_as_float(d[m][0]), ws[m][0], o0), x0, p[m][j][0]);
+                                        p[m][j][1] = fmaf(fmaf(__int_as_float(d[m][1]), ws[m][0], o0), x1, p[m][j][1]);
+                                        p[m][j][2] = fmaf(fmaf(__int_as_float(d[m][2]), ws[m][1], o1), x0, p[m][j][2]);
+                                        p[m][j][3] = fmaf(fmaf(__int_as_float(d[m][3]), ws[m][1], o1), x1, p[m][j][3]);
                                     }
                                 }
                             }
@@ -327,19 +329,22 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
 // ---- many rows: the integer tensor cores --------------------------------------------------------------------------------
 // A CTA computes 128 outputs (gated: 64 of each matrix) of RT rows over a range of inputs: D [128 outputs x RT rows] (int32, TMEM) =
 // W (int8, 128 inputs per stage) x^T by tcgen05.mma kind::i8, one product per group of GS inputs, exact.  Roles:
-//   warps 0 .. 7   drain: a thread owns an output (TMEM lane) and RT / 2 rows: p = fma(D, ws xs, p), packed over row pairs; ws in a
-//                  register, xs broadcast from shared memory; a slice's p, and the running total, rest in TMEM columns
-//   warps 8 .. 11  unpack: 32 bytes of a tile per load, straight from the layout (four chunks ahead in registers), to int8 rows of 128 inputs with
-//                  the 128-byte swizzle (K-major A operand); first thread: the rows' levels by TMA (K-major B operand); the xs
-//   warp 12        issues the MMAs, two D buffers in turn
-// What bounds it is the drain: per D value one conversion, a multiplication for the scales' product and a multiply-add, 128 of either per
-// clock and SM at most (64 conversions), against 4,096 or more products per clock in the tensor core.
+//   warps 0 .. 7    drain: a warp owns 32 outputs x RT / 2 rows in accumulator-fragment layout (4 outputs per thread: a scale read from
+//                   shared memory serves several values): p = fma(D ws, xs, p), packed over row pairs; the scales are staged by
+//                   these warps a slice ahead; the first slice of a pair rests in TMEM
+//   4 or 8 warps    unpack: a quarter of a chunk each, 1 KB of a tile per load, straight from the layout (registers, four steps ahead), to int8 rows of 128 inputs with
+//                   the 128-byte swizzle (K-major A operand); a chunk's first step also asks for the rows' levels by TMA (K-major B operand)
+//   one warp        issues the MMAs into two D buffers in turn, of as many groups as fill 128 columns (up to a chunk's)
+// What bounds it is the drain: per D value an addition, two multiply-adds and its part of the loads and waits, against 4,096 or more products per
+// clock in the tensor core; 16 warps, because two per scheduler left it waiting for TMEM loads most of the time.
 // With few tiles the inputs are split over the C CTAs of a cluster at multiples of 1,024: every CTA leaves the sums of its pairs of slices
 // in its shared memory and each CTA adds up its share of the rows in the one order, reading from the others'.
-constexpr int Q4T_THREADS = 416, Q4T_FS = 129;
+constexpr int Q4T_DRAIN = 8, Q4T_FS = 132, Q4T_BAND = 12;
+__host__ __device__ constexpr int q4t_unpack(int rt) { return rt == 128 ? 4 : 8; }  // unpack warps
+__host__ __device__ constexpr int q4t_threads(int rt) { return 32 * (Q4T_DRAIN + q4t_unpack(rt) + 1); }
 __host__ __device__ constexpr int q4t_stage(int rt) { return 16384 + rt * 128; }
-__host__ __device__ constexpr int q4t_xs(int gs, int rt) { return 2 * (Q4_SLICE / gs) * rt * 4; }
-__host__ __device__ constexpr int q4t_sums(int rt) { return rt * Q4T_FS * 4; }  // one pair's sums [RT][129]
+__host__ __device__ constexpr int q4t_scales(int gs, int rt) { return 2 * (Q4_SLICE / gs) * (rt + 128) * 4; }  // two slices' scales of the rows and of the outputs
+__host__ __device__ constexpr int q4t_sums(int rt) { return rt * Q4T_FS * 4; }  // one pair's sums [RT][132]
 
 __device__ __forceinline__ void ldg_stream8(const void *p, uint32_t *r) {
     asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -356,51 +361,82 @@ __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
+// Two adjacent rows of one output, as the halves of 64-bit registers (float2 values would be taken apart and put together again by moves):
+// p += round(D ws) xs for both rows, from the int32 sums d0, d1 (16 D); w2 = ws / 16 twice, o2 = -Q4_MAGIC_F w2.  The offset goes in by one
+// logic operation, (d & 0x7fffff) ^ 0x4B400000 (the sums fit 23 bits; flipping their sign bit adds 2^22): additions would be put on the pipe that
+// the multiply-adds need (630 against 530 clocks per 128 x 128 group in isolation).
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ void q4_add2(uint64_t &p, uint32_t d0, uint32_t d1, uint64_t w2, uint64_t o2, uint64_t x2) {
+    asm("{\n.reg .b32 a, b;\n.reg .b64 t;\nlop3.b32 a, %1, %6, %7, 0x6a;\nlop3.b32 b, %2, %6, %7, 0x6a;\nmov.b64 t, {a, b};\nfma.rn.f32x2 t, t, %3, %4;\nfma.rn.f32x2 %0, t, %5, %0;\n}"
+        : "+l"(p)
+        : "r"(d0), "r"(d1), "l"(w2), "l"(o2), "l"(x2), "r"(0x7fffffu), "r"(Q4_MAGIC));
+}
 
-// stages: operand stages; np: pairs of slices per CTA (C > 1: also the number of sums kept); grid (C, output tiles, row tiles), cluster (C, P)
+// lst: log2 of the operand stages; np: pairs of slices per CTA (C > 1: also the number of sums kept); clusters of C P CTAs
 template <int GS, int RT, bool GATED>
-__global__ void __launch_bounds__(Q4T_THREADS, 1)
-    q4_tiles_kernel(const Q4Args a, const __grid_constant__ CUtensorMap xmap, const int stages, const int np, const int C, const int P, int *err) {
-    constexpr int GC = Q4_CHUNK / GS, PER = Q4_SLICE / GS, RC = RT / 2, TILES = GATED ? 4 : 8;
-    constexpr int HOLD = 2 * RT, TOTAL = 3 * RT, COLS = 4 * RT;  // TMEM: two D buffers, a slice's p, the total
+__global__ void __launch_bounds__(q4t_threads(RT), 1)
+    q4_tiles_kernel(const Q4Args a, const __grid_constant__ CUtensorMap xmap, const int lst, const int np, const int C, const int P, int *err) {
+    constexpr int DW = Q4T_DRAIN, UW = q4t_unpack(RT), GC = Q4_CHUNK / GS, PER = Q4_SLICE / GS, RC = 4 * RT / DW, TILES = GATED ? 4 : 8;
+    constexpr int GB = GC < 128 / RT ? GC : 128 / RT, NB = GC / GB;  // groups per D buffer, buffers' worth per chunk
+    constexpr int UC = RC < 32 ? RC : 32, NU = UC / 8;  // rows drained at a time
+    constexpr int HOLD = 256, TOTAL = HOLD + RT;  // TMEM: two D buffers of 128 columns, a slice's p, the running total
+    constexpr int XE = (RT * PER + 32 * DW - 1) / (32 * DW);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float *xss = reinterpret_cast<float *>(sm + stages * q4t_stage(RT));  // [2][PER][RT]
-    float *sums = xss + q4t_xs(GS, RT) / 4;                              // [C > 1 ? np : 1][RT][129]
-    __shared__ __align__(8) uint64_t full[4], empty[4], dfull[2], dempty[2], xfull[2], xempty[2], done;
+    float *xss = reinterpret_cast<float *>(sm + (q4t_stage(RT) << lst));  // [2][PER][RT]
+    float *wss = xss + 2 * PER * RT;                                     // [2][PER][128]
+    float *sums = wss + 2 * PER * 128;                               // [C > 1 ? np : 1][RT][132]
+    __shared__ __align__(8) uint64_t full[4], empty[4], dfull[2], dempty[2], done;
     __shared__ uint32_t tmem_slot;
     __shared__ float top[RT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Q4View &W = a.w;
-    const int K = W.k, G = K / GS, row0 = blockIdx.z * RT, kc = blockIdx.x;
+    const int K = W.k, G = K / GS;
+    // a cluster is P adjacent tiles of C CTAs each along the inputs
+    const int kc = blockIdx.x % C, py = blockIdx.x / C % P, index = blockIdx.x / (C * P) * P + py;
+    // blocks in bands of Q4T_BAND output tiles, inside a band row tile by row tile: CTAs that run together share both operands' tiles evenly
+    const int fts = (W.tiles + TILES - 1) / TILES, rts = (a.rows + RT - 1) / RT;
+    const int band = index / (Q4T_BAND * rts), in = index - band * Q4T_BAND * rts, wide = min(Q4T_BAND, fts - band * Q4T_BAND);
+    const int ft = band * Q4T_BAND + in % wide, row0 = in / wide * RT;
     const int chunk0 = kc * np * (Q4_PAIR / Q4_CHUNK), chunk1 = min(W.chunks, chunk0 + np * (Q4_PAIR / Q4_CHUNK));
-    auto tile_of = [&](int tl) { return min((int)blockIdx.y * TILES + (GATED ? tl & 3 : tl), W.tiles - 1); };
+    auto tile_of = [&](int tl) { return min(ft * TILES + (GATED ? tl & 3 : tl), W.tiles - 1); };
 
+    // ---- unpack: warp u takes part u % 4 (tiles 2 part, 2 part + 1) of the chunks u / 4, u / 4 + UW / 4, ... of the range
+    const int u = warp - DW, part = u & 3, cu = u >> 2, chunks = chunk1 - chunk0;
+    constexpr int CU = UW / 4;
     uint32_t ring[4][2][8];
     const uint8_t *lv[2];
-    if (warp >= 8 && warp < 12) {
+    auto fetch = [&](int rel, int slot) {  // (a chunk behind the last: the last one's bytes, not used)
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int tl = (warp - 8) + 4 * i;
-            const Q4View &M = GATED && tl >= 4 ? a.up : a.w;
-            lv[i] = reinterpret_cast<const uint8_t *>(M.levels) + (size_t)tile_of(tl) * W.chunks * 1024 + (lane & 15) * 64 + (lane >> 4) * 32;
-        }
+        for (int i = 0; i < 2; i++) ldg_stream8(lv[i] + (size_t)min(rel, chunks - 1) * 1024, ring[slot][i]);
+    };
+    if (u >= 0 && u < UW) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            lv[i] = reinterpret_cast<const uint8_t *>((GATED && part >= 2 ? a.up : a.w).levels) + ((size_t)tile_of(2 * part + i) * W.chunks + chunk0) * 1024 + (lane & 15) * 64 +
+                    (lane >> 4) * 32;
         // (the weights are written once, when the matrix is made: their loads need not wait for the kernel before this one)
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                if (chunk0 + c < chunk1) ldg_stream8(lv[i] + (size_t)(chunk0 + c) * 1024, ring[c][i]);
+        for (int i = 0; i < 4; i++) fetch(cu + CU * i, i);
     }
     pdl_launch_dependents();
     if (tid == 0) {
-        for (int i = 0; i < 4; i++) mbar_init(full + i, 129), mbar_init(empty + i, 1);
-        for (int i = 0; i < 2; i++) mbar_init(dfull + i, 1), mbar_init(dempty + i, 8), mbar_init(xfull + i, 128), mbar_init(xempty + i, 8);
+        for (int i = 0; i < 4; i++) mbar_init(full + i, 5), mbar_init(empty + i, 1);
+        for (int i = 0; i < 2; i++) mbar_init(dfull + i, 1), mbar_init(dempty + i, DW);
         mbar_init(&done, 1);
         mbar_fence_init();
     }
-    if (warp == 12) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(COLS));
+    if (warp == DW + UW) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tc_fence_before();
@@ -409,191 +445,196 @@ __global__ void __launch_bounds__(Q4T_THREADS, 1)
     const uint32_t tbase = tmem_slot;
     pdl_wait();
 
-    if (warp < 8) {
-        // ---- drain
-        const int quad = warp & 3, col0 = (warp >> 2) * RC, tl = 2 * quad + (lane >> 4);
+    if (warp < DW) {
+        // ---- drain: the warp's 32 outputs x RC rows in accumulator-fragment layout, output 8 k + lane / 4, rows col0 + 8 i + 2 (lane % 4) + 0, 1
+        const int quad = warp & 3, col0 = (warp >> 2) * RC, g4 = lane >> 2, t2 = 2 * (lane & 3);
         const uint32_t mine = tbase + ((uint32_t)(quad * 32) << 16) + col0;
-        const Q4View &M = GATED && tl >= 4 ? a.up : a.w;
-        const __half *sc = M.scales + ((size_t)tile_of(tl) * W.slices * Q4_TILE + (lane & 15)) * PER;
-        float2 p[RC / 2];
+        constexpr int NI = RC / 8;
+        uint64_t p[4][NI];  // row pairs
         bool ok = true;
-        int gi = 0;  // groups drained
-        __align__(16) __half wsn[PER], wsc[PER];
-        auto fetch_ws = [&](int sl) {
-            const __half *s = sc + (size_t)sl * Q4_TILE * PER;
-            if constexpr (PER == 4) *reinterpret_cast<uint2 *>(wsn) = __ldg(reinterpret_cast<const uint2 *>(s));
-            else
-#pragma unroll
-                for (int i = 0; i < PER / 8; i++) reinterpret_cast<uint4 *>(wsn)[i] = __ldg(reinterpret_cast<const uint4 *>(s) + i);
-        };
+        int buf = 0;
+        uint32_t ph = 0;  // the next D buffer and the phase of its barrier
         const int sl0 = chunk0 / 4, sl1 = (chunk1 + 3) / 4;
-        fetch_ws(sl0);
-        for (int sl = sl0; sl < sl1 && ok; sl++) {
-            const int slot = (sl - sl0) & 1;
+        // The scales of a slice, a slice ahead: loaded into registers (from clamped addresses, so that nothing waits for the loads before
+        // they are stored) and stored to shared memory when the slice before is done.  Rows: element e = (row e / PER, group e % PER);
+        // outputs: four groups of one output per thread, times 1 / 16 (the levels are in the upper halves of their bytes).
+        constexpr int XW = (128 * (PER / 4) + 32 * DW - 1) / (32 * DW), WT = 32 * DW / (PER / 4);
+        float xn[XE];
+        uint2 wn[XW];
+        const int wf = tid / (PER / 4), wp = tid % (PER / 4) * 4;  // outputs wf + WT i (where there are), first of their groups
+        const __half *wsrc[XW];
 #pragma unroll
-            for (int i = 0; i < PER; i++) wsc[i] = wsn[i];
-            if (sl + 1 < sl1) fetch_ws(sl + 1);
+        for (int i = 0; i < XW; i++) {
+            const int f = min(wf + WT * i, 127);
+            wsrc[i] = (GATED && f >= 64 ? a.up : a.w).scales + ((size_t)tile_of(f >> 4) * W.slices * Q4_TILE + (f & 15)) * PER + wp;
+        }
+        auto fetch_scales = [&](int sl) {
 #pragma unroll
-            for (int i = 0; i < RC / 2; i++) p[i] = make_float2(0.0f, 0.0f);
-            ok = mbar_wait_bounded_quiet(xfull + slot, (uint32_t)((sl - sl0) >> 1) & 1u, err, 81);
-            const float *xsl = xss + slot * PER * RT + col0;
+            for (int i = 0; i < XE; i++) {
+                const int e = i * 32 * DW + tid;
+                xn[i] = __ldg(a.xs + (size_t)min(row0 + e / PER, a.rows - 1) * G + min(sl * PER + e % PER, G - 1));
+            }
 #pragma unroll
-            for (int g = 0; g < PER; g++) {
-                if (4 * sl + g / GC < chunk1 && ok) {
-                    const int buf = gi & 1;
-                    ok = mbar_wait_bounded_quiet(dfull + buf, (uint32_t)(gi >> 1) & 1u, err, 82);
-                    ok = __all_sync(0xffffffffu, ok);
-                    tc_fence_after();
-                    const float w = __half2float(wsc[g]) * 0.0625f;  // (1 / 16: the levels are in the upper halves of their bytes)
-                    const float2 w2 = make_float2(w, w);
-                    constexpr int B = RC < 32 ? RC : 32;  // columns read at a time
+            for (int i = 0; i < XW; i++) wn[i] = __ldg(reinterpret_cast<const uint2 *>(wsrc[i] + (size_t)sl * Q4_TILE * PER));
+        };
+        auto put_scales = [&](int sl, int slot) {
 #pragma unroll
-                    for (int c = 0; c < RC; c += B) {
-                        uint32_t r[B];
-                        if constexpr (B == 16) tmem_ld16(mine + buf * RT, r);
-                        else tmem_ld32(mine + buf * RT + c, r);
+            for (int i = 0; i < XE; i++) {
+                const int e = i * 32 * DW + tid;
+                if (e < RT * PER) xss[(slot * PER + e % PER) * RT + e / PER] = row0 + e / PER < a.rows && sl * PER + e % PER < G ? xn[i] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < XW; i++)
+                if (wf + WT * i < 128) {
+                    const float2 lo = __half22float2(*reinterpret_cast<__half2 *>(&wn[i].x)), hi = __half22float2(*reinterpret_cast<__half2 *>(&wn[i].y));
+                    float *o = wss + (slot * PER + wp) * 128 + wf + WT * i;
+                    o[0] = lo.x * 0.0625f, o[128] = lo.y * 0.0625f, o[256] = hi.x * 0.0625f, o[384] = hi.y * 0.0625f;
+                }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * DW) : "memory");
+        };
+        fetch_scales(sl0);
+        put_scales(sl0, 0);
+        for (int sl = sl0; sl < sl1; sl++) {
+            const int slot = (sl - sl0) & 1, bufs = min(4, chunk1 - 4 * sl) * NB;
+            if (sl + 1 < sl1) fetch_scales(sl + 1);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < NI; i++) p[k][i] = 0;
+            const float *xsl = xss + slot * PER * RT + col0 + t2, *wsl = wss + slot * PER * 128 + quad * 32 + g4;
+#pragma unroll 1
+            for (int b = 0; b < bufs; b++) {
+                if (ok) ok = mbar_wait_bounded_quiet(dfull + buf, ph, err, 82);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_fence_after();
+#pragma unroll
+                for (int g = 0; g < GB; g++) {
+                    const int at = b * GB + g;
+                    uint64_t w2[4], o2[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float w = wsl[at * 128 + 8 * k], o = -Q4_MAGIC_F * w;
+                        w2[k] = pack2(w, w), o2[k] = pack2(o, o);
+                    }
+#pragma unroll
+                    for (int c = 0; c < RC; c += UC) {
+                        uint32_t r[2][4 * NU];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) tmem_ld_frag<NU>(mine + ((uint32_t)(16 * h) << 16) + buf * 128 + g * RT + c, r[h]);
+                        uint64_t x2[NU];
+#pragma unroll
+                        for (int i = 0; i < NU; i++) x2[i] = *reinterpret_cast<const uint64_t *>(xsl + at * RT + c + 8 * i);
                         tmem_wait_ld();
-                        if (c + B == RC) {
+                        if (g == GB - 1 && c + UC == RC) {
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(dempty + buf);
                         }
 #pragma unroll
-                        for (int j = 0; j < B; j += 4) {
-                            const float4 x = *reinterpret_cast<const float4 *>(xsl + g * RT + c + j);
-                            float2 &p0 = p[(c + j) / 2], &p1 = p[(c + j) / 2 + 1];
-                            p0 = __ffma2_rn(make_float2((float)(int)r[j], (float)(int)r[j + 1]), __fmul2_rn(w2, make_float2(x.x, x.y)), p0);
-                            p1 = __ffma2_rn(make_float2((float)(int)r[j + 2], (float)(int)r[j + 3]), __fmul2_rn(w2, make_float2(x.z, x.w)), p1);
-                        }
+                        for (int i = 0; i < NU; i++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) q4_add2(p[k][c / 8 + i], r[k >> 1][4 * i + 2 * (k & 1)], r[k >> 1][4 * i + 2 * (k & 1) + 1], w2[k], o2[k], x2[i]);
                     }
-                    gi++;
                 }
+                buf ^= 1, ph ^= buf == 0;
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(xempty + slot);
-            // the end of the slice: hold p, or add it to the slice before and the pair to the total
-            if (!(sl & 1) && sl + 1 < sl1) {
-                if constexpr (RC == 16) tmem_st16(mine + HOLD, reinterpret_cast<uint32_t *>(p));
-                else
+            // the end of the slice: hold p, or add it to the slice before and keep the pair (C > 1) or add it to the total
+            constexpr int NE = NI < 4 ? NI : 4;  // pieces of 8 NE rows
+            const int pair = (sl - sl0) >> 1;
+            const bool hold = !(sl & 1) && sl + 1 < sl1, more = C == 1 && pair > 0, store = !hold && (C > 1 || sl + 1 == sl1);
 #pragma unroll
-                    for (int i = 0; i < RC / 32; i++) tmem_st32(mine + HOLD + 32 * i, reinterpret_cast<uint32_t *>(p) + 32 * i);
-                tmem_wait_st();
-            } else {
-                const int pair = (sl - sl0) >> 1;
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < RC / 16; i++) {
-                    uint32_t r[16];
-                    if (sl & 1) {
-                        tmem_ld16(mine + HOLD + 16 * i, r);
+                for (int c = 0; c < NI; c += NE) {
+                    const uint32_t at = mine + ((uint32_t)(16 * h) << 16) + 8 * c;
+                    uint32_t q[4 * NE];
+                    auto plus = [&](uint32_t from) {
+                        tmem_ld_frag<NE>(from, q);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            p[8 * i + j] = __fadd2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), p[8 * i + j]);
-                    }
-                    if (C == 1) {
-                        if (pair > 0) {
-                            tmem_ld16(mine + TOTAL + 16 * i, r);
-                            tmem_wait_ld();
-                        } else {
+                        for (int i = 0; i < NE; i++)
 #pragma unroll
-                            for (int j = 0; j < 16; j++) r[j] = 0u;
-                        }
+                            for (int k = 0; k < 2; k++) {
+                                uint64_t &v = p[2 * h + k][c + i];
+                                asm volatile("{\n.reg .b64 t;\nmov.b64 t, {%1, %2};\nadd.rn.f32x2 %0, t, %0;\n}" : "+l"(v) : "r"(q[4 * i + 2 * k]), "r"(q[4 * i + 2 * k + 1]));
+                            }
+                    };
+                    if (!hold && (sl & 1)) plus(at + HOLD);
+                    if (!hold && more) plus(at + TOTAL);
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            p[8 * i + j] = __fadd2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), p[8 * i + j]);
-                        if (sl + 1 < sl1) {
-                            tmem_st16(mine + TOTAL + 16 * i, reinterpret_cast<uint32_t *>(p + 8 * i));
-                            tmem_wait_st();
-                        }
-                    }
-                }
-                if (C > 1 || sl + 1 == sl1) {
-                    float *o = sums + ((size_t)(C > 1 ? pair : 0) * RT + col0) * Q4T_FS + quad * 32 + lane;
+                    for (int i = 0; i < NE; i++)
 #pragma unroll
-                    for (int j = 0; j < RC / 2; j++) {
-                        o[2 * j * Q4T_FS] = p[j].x;
-                        o[(2 * j + 1) * Q4T_FS] = p[j].y;
+                        for (int k = 0; k < 2; k++) q[4 * i + 2 * k] = (uint32_t)p[2 * h + k][c + i], q[4 * i + 2 * k + 1] = (uint32_t)(p[2 * h + k][c + i] >> 32);
+                    if (!store) tmem_st_frag<NE>(at + (hold ? HOLD : TOTAL), q);
+                    else {
+                        float *o = sums + ((size_t)(C > 1 ? pair : 0) * RT + col0 + 8 * c + t2) * Q4T_FS + quad * 32 + 16 * h + g4;
+#pragma unroll
+                        for (int i = 0; i < 4 * NE; i++) o[(8 * (i >> 2) + (i & 1)) * Q4T_FS + 8 * ((i >> 1) & 1)] = __uint_as_float(q[i]);
                     }
                 }
-            }
+            tmem_wait_st();
+            if (sl + 1 < sl1) put_scales(sl + 1, slot ^ 1);
         }
-    } else if (warp < 12) {
-        // ---- unpack
-        const int u = tid - 256, f = lane & 15, h = lane >> 4, row = row0 + u;
+    } else if (u < UW) {
         bool ok = true;
-        float xn[PER];
-        auto fetch_xs = [&](int sl) {
+        const int f = lane & 15, h = lane >> 4;
+        uint8_t *out[4];  // the lane's four 16-byte places in the first tile of its part
 #pragma unroll
-            for (int i = 0; i < PER; i++) xn[i] = u < RT && row < a.rows && sl * PER + i < G ? __ldg(a.xs + (size_t)row * G + sl * PER + i) : 0.0f;
-        };
-        fetch_xs(chunk0 / 4);
-        int st = 0;
-        uint32_t ph = 0;  // the phase of the stages' empty barriers that the next round waits for
-        for (int base = chunk0; base < chunk1 && ok; base += 4) {
-            const int sl = base / 4, n = sl - chunk0 / 4;
-            if (n >= 2) ok = mbar_wait_bounded_quiet(xempty + (n & 1), (uint32_t)((n >> 1) - 1) & 1u, err, 83);
-            if (u < RT)
+        for (int s = 0; s < 4; s++) out[s] = sm + part * 4096 + f * 128 + (((2 * s + h) ^ (f & 7)) << 4);
+        for (int r0 = cu; r0 < chunks && ok; r0 += 4 * CU) {
 #pragma unroll
-                for (int i = 0; i < PER; i++) xss[((n & 1) * PER + i) * RT + u] = xn[i];
-            mbar_arrive(xfull + (n & 1));
-            if (base + 4 < chunk1) fetch_xs(sl + 1);
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int chunk = base + c;
-                if (chunk < chunk1 && ok) {
-                    uint8_t *A = sm + st * q4t_stage(RT);
-                    if (chunk - chunk0 >= stages) ok = mbar_wait_bounded_quiet(empty + st, ph ^ 1u, err, 84);
-                    if (u == 0) {
+            for (int i = 0; i < 4; i++) {
+                const int rel = r0 + CU * i, st = rel & ((1 << lst) - 1);
+                if (rel < chunks && ok) {
+                    const int at = st * q4t_stage(RT);
+                    if (rel >> lst) ok = mbar_wait_bounded_quiet(empty + st, (uint32_t)((rel >> lst) - 1) & 1u, err, 84);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (part == 0 && lane == 0 && ok) {
                         mbar_expect_tx(full + st, RT * 128);
-                        tma_load_2d(A + 16384, &xmap, chunk * Q4_CHUNK, row0, full + st);
+                        tma_load_2d(sm + at + 16384, &xmap, (chunk0 + rel) * Q4_CHUNK, row0, full + st);
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        uint8_t *o = A + ((warp - 8) + 4 * i) * 2048 + f * 128;
+                    for (int t = 0; t < 2; t++)
 #pragma unroll
                         for (int s = 0; s < 4; s++) {
-                            const uint32_t w0 = ring[c][i][s], w1 = ring[c][i][4 + s];
-                            *reinterpret_cast<uint4 *>(o + (((2 * s + h) ^ (f & 7)) << 4)) =
-                                make_uint4((w0 << 4) & 0xF0F0F0F0u, w0 & 0xF0F0F0F0u, (w1 << 4) & 0xF0F0F0F0u, w1 & 0xF0F0F0F0u);
+                            const uint32_t w0 = ring[i][t][s], w1 = ring[i][t][4 + s];
+                            *reinterpret_cast<uint4 *>(out[s] + at + t * 2048) = make_uint4((w0 << 4) & 0xF0F0F0F0u, w0 & 0xF0F0F0F0u, (w1 << 4) & 0xF0F0F0F0u, w1 & 0xF0F0F0F0u);
                         }
-                        if (chunk + 4 < chunk1) ldg_stream8(lv[i] + (size_t)(chunk + 4) * 1024, ring[c][i]);
-                    }
+                    fetch(rel + 4 * CU, i);
                     fence_proxy_async();
-                    mbar_arrive(full + st);
-                    if (++st == stages) st = 0, ph ^= 1u;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + st);
                 }
             }
         }
-        if (u == 0 && *reinterpret_cast<volatile int *>(err) != 0)  // a wait ran out: the copies in flight get a bounded time to land
-            for (int i = 0; i < stages; i++) mbar_drain(full + i, ph);
+        if (lane == 0 && *reinterpret_cast<volatile int *>(err) != 0)  // a wait ran out: the copies in flight get a bounded time to land
+            for (int i = 0; i < (1 << lst); i++) mbar_drain(full + i, 0), mbar_drain(full + i, 1);
     } else if (elect_one()) {
         // ---- MMA issue
         constexpr uint32_t idesc = umma_idesc_i8(128, RT, 0, 0, 1, 1);
         const uint32_t sbase = smem_u32(sm);
-        int st = 0, gi = 0;
-        uint32_t ph = 0;
+        int buf = 0;
+        uint32_t ph = 1;  // the phase of the D buffer's barrier before its last release (the first round does not wait)
         bool ok = true;
         for (int chunk = chunk0; chunk < chunk1 && ok; chunk++) {
-            ok = mbar_wait_bounded_quiet(full + st, ph, err, 85);
-            tc_fence_after();
+            const int rel = chunk - chunk0, st = rel & ((1 << lst) - 1);
+            ok = mbar_wait_bounded_quiet(full + st, (uint32_t)(rel >> lst) & 1u, err, 85);
             const uint32_t A = sbase + st * q4t_stage(RT), B = A + 16384;
 #pragma unroll
-            for (int gc = 0; gc < GC; gc++) {
-                const int buf = gi & 1;
-                if (gi >= 2 && ok) ok = mbar_wait_bounded_quiet(dempty + buf, (uint32_t)((gi >> 1) - 1) & 1u, err, 86);
+            for (int b = 0; b < NB; b++) {
+                if (ok && (rel * NB + b >= 2)) ok = mbar_wait_bounded_quiet(dempty + buf, ph, err, 86);
                 if (ok) {
                     tc_fence_after();
 #pragma unroll
-                    for (int s = 0; s < GS / 32; s++) {
-                        const int at = gc * GS + 32 * s;
-                        umma_i8(tbase + buf * RT, umma_desc(A + at, 16, 1024, 2), umma_desc(B + at, 16, 1024, 2), idesc, s > 0);
+                    for (int s = 0; s < GB * GS / 32; s++) {
+                        const int at = b * GB * GS + 32 * s;
+                        umma_i8(tbase + buf * 128 + s / (GS / 32) * RT, umma_desc(A + at, 16, 1024, 2), umma_desc(B + at, 16, 1024, 2), idesc, s % (GS / 32) > 0);
                     }
                     umma_commit(dfull + buf);
+                    buf ^= 1, ph ^= buf == 0;
                 }
-                gi++;
             }
             umma_commit(empty + st);
-            if (++st == stages) st = 0, ph ^= 1u;
         }
         umma_commit(&done);
         mbar_drain(&done, 0);  // (no MMA and no arrival of one is in flight when the CTA ends)
@@ -601,13 +642,13 @@ __global__ void __launch_bounds__(Q4T_THREADS, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(COLS));
+    if (warp == DW + UW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512));
     if (C > 1) cluster_sync_all();  // (the clusters of 128-wide groups and C = 1 have nothing to read here yet)
 
     // ---- the totals of this CTA's share of the rows, a warp per row, lanes along the outputs
     const int share = (RT + C - 1) / C, r0 = kc * share, r1 = min(min(r0 + share, RT), a.rows - row0);
     const int pairs = (W.chunks + 7) / 8;
-    const uint32_t prank = (uint32_t)(blockIdx.y % P) * C;
+    const uint32_t prank = (uint32_t)py * C;
     auto total = [&](int r, int f) {
         if (C == 1) return sums[r * Q4T_FS + f];
         float t = 0.0f;
@@ -615,17 +656,17 @@ __global__ void __launch_bounds__(Q4T_THREADS, 1)
         return t;
     };
     if constexpr (!GATED) {
-        for (int r = r0 + warp; r < r1; r += Q4T_THREADS / 32)
+        for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int f = blockIdx.y * 128 + 32 * i + lane;
+                const int f = ft * 128 + 32 * i + lane;
                 const float v = total(r, 32 * i + lane);
                 if (f < W.n) a.out[(size_t)(row0 + r) * W.n + f] = v;
             }
     } else {
         for (int pass = a.hq && GS == 128 ? 0 : 1; pass < 2; pass++) {
             if (pass == 1 && a.hq && GS == 128) cluster_sync_all();  // the two CTAs of a group's halves have their maxima
-            for (int r = r0 + warp; r < r1; r += Q4T_THREADS / 32) {
+            for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32) {
                 float v[2];
                 uint32_t m[2];
 #pragma unroll
@@ -639,12 +680,12 @@ __global__ void __launch_bounds__(Q4T_THREADS, 1)
                     continue;
                 }
                 if (a.hq && GS == 128) {
-                    const uint32_t other = (uint32_t)(blockIdx.y % P ^ 1) * C + kc;
+                    const uint32_t other = (uint32_t)(py ^ 1) * C + kc;
                     m[0] = m[1] = max(m[0], __float_as_uint(ld_cluster(top + r, other)));
                 }
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int f = blockIdx.y * 64 + 32 * i + lane;
+                    const int f = ft * 64 + 32 * i + lane;
                     const size_t at = (size_t)(row0 + r) * W.n + f;
                     if (f < W.n) {
                         if (a.out) a.out[at] = v[i];
@@ -665,11 +706,10 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
     const int pairs = (a.w.slices + 1) / 2, np = (pairs + C - 1) / C;
     C = (pairs + np - 1) / np;
     const int P = GATED && a.hq && GS == 128 ? 2 : 1;
-    const int fixed = 1024 + q4t_xs(GS, RT) + q4t_sums(RT) * (C > 1 ? np : 1), most = 226 * 1024;
-    int stages = (most - fixed) / q4t_stage(RT);
-    if (stages < 2) return cudaErrorInvalidValue;
-    if (stages > 4) stages = 4;
-    const int smem = fixed + stages * q4t_stage(RT);
+    const int fixed = 1024 + q4t_scales(GS, RT) + q4t_sums(RT) * (C > 1 ? np : 1), most = 226 * 1024;
+    const int lst = (most - fixed) / q4t_stage(RT) >= 4 ? 2 : 1;
+    const int smem = fixed + (q4t_stage(RT) << lst);
+    if (smem > most) return cudaErrorInvalidValue;
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)a.w.k, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.w.k};
     const cuuint32_t box[2] = {Q4_CHUNK, RT}, es[2] = {1, 1};
@@ -681,20 +721,21 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     const int tiles = GATED ? 4 : 8;
-    cfg.gridDim = dim3(C, (a.w.tiles + tiles - 1) / tiles, (a.rows + RT - 1) / RT);
-    cfg.blockDim = dim3(Q4T_THREADS);
+    const int fts = (a.w.tiles + tiles - 1) / tiles, rts = (a.rows + RT - 1) / RT;
+    cfg.gridDim = dim3((unsigned)(C * fts * rts));
+    cfg.blockDim = dim3(q4t_threads(RT));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = C;
-    at[1].val.clusterDim.y = P;
+    at[1].val.clusterDim.x = C * P;
+    at[1].val.clusterDim.y = 1;
     at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = C * P > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, a, map, stages, np, C, P, err);
+    return cudaLaunchKernelEx(&cfg, kern, a, map, lst, np, C, P, err);
 }
 
 // Which rows per tile and how many CTAs along the inputs: the least estimated time, in clocks.  A group costs a CTA its drain (measured:
@@ -711,7 +752,7 @@ inline Q4Plan q4_plan(const Q4Args &a, bool gated, int n_sm) {
         for (int c = 1; c * P <= 8 && c <= pairs; c++) {
             const int np = (pairs + c - 1) / c;
             if ((pairs + np - 1) / np != c) continue;
-            if (1024 + q4t_xs(a.w.gs, rt) + q4t_sums(rt) * (c > 1 ? np : 1) + 2 * q4t_stage(rt) > 226 * 1024) continue;
+            if (1024 + q4t_scales(a.w.gs, rt) + q4t_sums(rt) * (c > 1 ? np : 1) + 2 * q4t_stage(rt) > 226 * 1024) continue;
             const long long ctas = (long long)c * tiles * ((a.rows + rt - 1) / rt), slots = n_sm / (c * P) * (c * P);
             const double time = (double)((ctas + slots - 1) / slots) * (3000.0 + (c > 1 ? 1500.0 : 0.0) + (double)np * (Q4_PAIR / a.w.gs) * group);
             if (time < least) least = time, best = {rt, c};
