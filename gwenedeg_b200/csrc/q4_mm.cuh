@@ -92,176 +92,209 @@ __device__ __forceinline__ uint4 ldg_stream(const uint4 *p) {
 }
 __device__ __forceinline__ void mma_s8(int *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_first(int *d, const uint32_t *a, uint32_t b0, uint32_t b1, int c) {  // (d need not be set to c first)
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c));
 }
 // An int32 sum S plus the bits of 1.5 2^23 are the bits of the float 1.5 2^23 + S, exactly, while |S| < 2^22 (here S = 16 D, as the levels
-// sit in the upper halves of their bytes: |S| <= 16 . 128 . 8 . 128 = 2^21).  With v = ws / 16, M = 1.5 2^23:  fma(M + S, v, -M v) =
-// round(D ws): M v is exact (ws has 11 significant bits), so one multiply-add converts, removes the offset and applies the weight's
-// scale, with the one rounding of the product.
+// sit in the upper halves of their bytes: |S| <= 16 . 128 . 8 . 128 = 2^21).  With M = 1.5 2^23:  fma(M + S, ws, -M ws) = round(S ws): M ws is
+// exact (ws has 11 significant bits), so one multiply-add converts, removes the offset and applies the weight's scale, with the one rounding
+// of the product.  The factor 16 is carried to the end, where the total is multiplied by 1 / 16 (both exact).
 constexpr int Q4_MAGIC = 0x4B400000;
 constexpr float Q4_MAGIC_F = 12582912.0f;
 
 // h = g sigmoid(g) u
 __device__ __forceinline__ float q4_silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
-// The simple kernel, right for every size: a CTA of NW warps computes 16 MT outputs (gated: 16 outputs of each matrix) of 8 NT rows, warp
-// w takes the slices w, w + NW, ...; weights go from global memory straight into the registers of the lane that feeds them to
-// mma.m16n8k32 (outputs as M, rows as N), the rows' levels come through L1.  The slices' partial sums meet in shared memory and are
-// added in order by the threads that own the outputs.
-template <int GS, int MT, int NT, bool GATED>
-__global__ void __launch_bounds__(256) q4_rows_kernel(const Q4Args a) {
+// ---- few rows: weights straight from memory into the registers that feed mma.m16n8k32 ------------------------------------
+__device__ __forceinline__ void cp_async16(void *dst, const void *src, bool valid) {  // (not valid: zeros, nothing is read)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void *dst, const void *src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+// A CTA of NW warps computes 16 outputs (gated: of each matrix) of 8 NT rows; warp w takes the slices w, w + NW, ...  Everything a slice
+// needs is asked for before its first product: its weights (a ring of one slice of one matrix in registers, 16-byte loads that are contiguous
+// over the warp; what comes next, the other matrix or the next slice, is asked for as the ring is used), the weights' scales, and the rows'
+// levels and scales (cp.async into the warp's own part of shared memory, rows 544 bytes apart: conflict-free 8-byte reads).  Outputs are M
+// of the MMA, rows N.  The slices' partial sums meet in shared memory and are added in order by the threads that own the outputs.
+// Bound by the weights' bytes; the weights' loads do not wait for the kernel before this one (they are constant), so they overlap its end.
+// Measured: 65536 x 4096 (groups of 64), one row, 24.9 us = 5.7 TB/s; walking over tiles with resident CTAs instead of one CTA per tile took
+// 47 us, prefetching a later CTA's weights into the L2 cache 31 us.
+constexpr int Q4R_XROW = Q4_SLICE + 32;  // bytes from row to row of a slice's levels
+__host__ __device__ constexpr int q4r_warp_bytes(int gs, int nt) { return 8 * nt * (Q4R_XROW + Q4_SLICE / gs * 4); }
+
+// MULTI: more slices than warps
+template <int GS, int NT, bool GATED, bool MULTI>
+__global__ void __launch_bounds__(256, NT == 1 && GS >= 64 ? 3 : NT <= 2 ? 2 : 1) q4_rows_kernel(const Q4Args a) {
     constexpr int GC = Q4_CHUNK / GS;        // groups per chunk
     constexpr int PER = Q4_SLICE / GS;       // groups per slice
-    constexpr int FT = 16 * MT, FS = FT + 4;  // outputs of the CTA, and their stride in shared memory (conflict-free stores)
+    constexpr int J = GATED ? 2 : 1;         // matrices
+    constexpr int FT = 16 * J, FS = FT + 4;  // outputs of the CTA, and their stride in shared memory (conflict-free stores)
     constexpr int R = 8 * NT;
-    extern __shared__ float red[];  // [NW][R][FS]
+    extern __shared__ __align__(16) uint8_t rows_smem[];  // per warp: levels [R][544], scales [PER][R]; its partial sums [R][FS] over the levels
     const int NW = blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int row0 = blockIdx.y * R, rows = min(a.rows - row0, R);
     const Q4View &W = a.w;
     const int K = W.k, G = K / GS;
+    uint8_t *xl = rows_smem + (size_t)w * q4r_warp_bytes(GS, NT);
+    float *xsm = reinterpret_cast<float *>(xl + R * Q4R_XROW);
+    auto red = [&](int u) { return reinterpret_cast<float *>(rows_smem + (size_t)u * q4r_warp_bytes(GS, NT)); };
 
-    const uint4 *lv[MT];
-    const __half *sc[MT];
+    const size_t at_levels = (size_t)blockIdx.x * W.chunks * 64 + lane, at_scales = ((size_t)blockIdx.x * W.slices * Q4_TILE + g) * PER;
+    uint4 ring[4][2];
+    auto fetch = [&](const Q4View &M, int chunk, int slot) {  // (behind the end: the last chunk's bytes, not used)
+        chunk = min(chunk, W.chunks - 1);
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const Q4View &M = GATED && m == 1 ? a.up : a.w;
-        const size_t tile = GATED ? blockIdx.x : min((int)blockIdx.x * MT + m, W.tiles - 1);
-        lv[m] = M.levels + tile * W.chunks * 64 + lane;
-        sc[m] = M.scales + tile * W.slices * Q4_TILE * PER + g * PER;
-    }
-    uint4 ring[4][MT][2];
-    auto fetch = [&](int chunk, int slot) {
+        for (int h = 0; h < 2; h++) ring[slot][h] = ldg_stream(M.levels + at_levels + (size_t)chunk * 64 + h * 32);
+    };
+    union Scales {  // of one output in a slice
+        uint2 v[PER / 4];
+        __half h[PER];
+    } ws[2], wn[2];
+    auto fetch_ws = [&](const Q4View &M, int sl) {
+        sl = min(sl, W.slices - 1);
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-                ring[slot][m][h] = chunk < W.chunks ? ldg_stream(lv[m] + (size_t)chunk * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < PER / 4; i++) wn[h].v[i] = __ldg(reinterpret_cast<const uint2 *>(M.scales + at_scales + ((size_t)sl * Q4_TILE + 8 * h) * PER) + i);
     };
     // (the weights are written once, when the matrix is made: their loads need not wait for the kernel before this one)
 #pragma unroll
-    for (int c = 0; c < 4; c++) fetch(4 * w + c, c);
+    for (int c = 0; c < 4; c++) fetch(a.w, 4 * w + c, c);
+    fetch_ws(a.w, w);
     pdl_launch_dependents();
     pdl_wait();
 
-    const int8_t *xr[NT];
+    constexpr int OWN = R * FT / 128 > 0 ? R * FT / 128 : 1;
+    float tot[OWN];
 #pragma unroll
-    for (int j = 0; j < NT; j++) xr[j] = a.xq + (size_t)(row0 + min(8 * j + g, rows - 1)) * K + 8 * t;
-    float tot[R * FT / 128 > 0 ? R * FT / 128 : 1];
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(tot) / 4); i++) tot[i] = 0.0f;
+    for (int i = 0; i < OWN; i++) tot[i] = 0.0f;
 
-    for (int s0 = 0; s0 < W.slices; s0 += NW) {
+    for (int s0 = 0; s0 < (MULTI ? W.slices : 1); s0 += NW) {
         const int sl = s0 + w;
-        float p[MT][NT][4];
+        float p[J][NT][4];  // output g of rows 2 t, 2 t + 1; output g + 8 of the same
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int m = 0; m < J; m++)
 #pragma unroll
-            for (int j = 0; j < NT; j++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[m][j][i] = 0.0f;
+            for (int j = 0; j < NT; j++) p[m][j][0] = p[m][j][1] = p[m][j][2] = p[m][j][3] = 0.0f;
+        if (s0 > 0) __syncthreads();  // the last round's partial sums have been read
         if (sl < W.slices) {
-            const __half *ss[MT];
+            const int k0 = sl * Q4_SLICE + 16 * lane;
 #pragma unroll
-            for (int m = 0; m < MT; m++) ss[m] = sc[m] + (size_t)sl * Q4_TILE * PER;
+            for (int r = 0; r < R; r++)
+                if (r < rows) cp_async16(xl + r * Q4R_XROW + 16 * lane, a.xq + (size_t)(row0 + r) * K + min(k0, K - 16), k0 < K);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int chunk = 4 * sl + c;
-                if (chunk < W.chunks) {
+            for (int i = 0; i < R * PER / 32; i++) {
+                const int e = 32 * i + lane, r = e / PER, gr = sl * PER + e % PER;
+                if (r < rows) cp_async4(xsm + (e % PER) * R + r, a.xs + (size_t)(row0 + r) * G + min(gr, G - 1), gr < G);
+            }
+            if (s0 > 0) fetch_ws(a.w, sl);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
 #pragma unroll
-                    for (int gc = 0; gc < GC; gc++) {
-                        const int grp = chunk * GC + gc;
-                        if (grp < G) {
-                            uint32_t A[MT][GS / 32][4];
-                            float ws[MT][2];
+            for (int m = 0; m < J; m++) {
 #pragma unroll
-                            for (int m = 0; m < MT; m++) {
+                for (int h = 0; h < 2; h++) ws[h] = wn[h];
+                if (m + 1 < J) fetch_ws(a.up, sl);
 #pragma unroll
-                                for (int st = 0; st < GS / 32; st++) {
-                                    const int s = gc * (GS / 32) + st;
-                                    const uint32_t lo = s == 0 ? ring[c][m][0].x : s == 1 ? ring[c][m][0].y : s == 2 ? ring[c][m][0].z : ring[c][m][0].w;
-                                    const uint32_t hi = s == 0 ? ring[c][m][1].x : s == 1 ? ring[c][m][1].y : s == 2 ? ring[c][m][1].z : ring[c][m][1].w;
-                                    A[m][st][0] = (lo << 4) & 0xF0F0F0F0u;
-                                    A[m][st][1] = (hi << 4) & 0xF0F0F0F0u;
-                                    A[m][st][2] = lo & 0xF0F0F0F0u;
-                                    A[m][st][3] = hi & 0xF0F0F0F0u;
-                                }
-                                ws[m][0] = __half2float(ss[m][c * GC + gc]) * 0.0625f;
-                                ws[m][1] = __half2float(ss[m][8 * PER + c * GC + gc]) * 0.0625f;
+                for (int c = 0; c < 4; c++) {
+                    // (a chunk at a time: without this the compiler unpacks and converts everything ahead and runs out of registers)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        asm volatile("" : "+r"(ring[c][h].x), "+r"(ring[c][h].y), "+r"(ring[c][h].z), "+r"(ring[c][h].w)::"memory");
+#pragma unroll
+                    for (int i = 0; i < PER / 2; i++) asm volatile("" : "+r"(ws[i & 1].v[i >> 1].x), "+r"(ws[i & 1].v[i >> 1].y));
+                    if (4 * sl + c < W.chunks) {
+#pragma unroll
+                        for (int gc = 0; gc < GC; gc++) {
+                            uint32_t A[GS / 32][4];
+                            float wf[2], of[2];
+#pragma unroll
+                            for (int st = 0; st < GS / 32; st++) {
+                                const int s = gc * (GS / 32) + st;
+                                const uint32_t lo = s == 0 ? ring[c][0].x : s == 1 ? ring[c][0].y : s == 2 ? ring[c][0].z : ring[c][0].w;
+                                const uint32_t hi = s == 0 ? ring[c][1].x : s == 1 ? ring[c][1].y : s == 2 ? ring[c][1].z : ring[c][1].w;
+                                A[st][0] = (lo << 4) & 0xF0F0F0F0u;
+                                A[st][1] = (hi << 4) & 0xF0F0F0F0u;
+                                A[st][2] = lo & 0xF0F0F0F0u;
+                                A[st][3] = hi & 0xF0F0F0F0u;
+                            }
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                wf[h] = __half2float(ws[h].h[c * GC + gc]);
+                                of[h] = -Q4_MAGIC_F * wf[h];
                             }
 #pragma unroll
                             for (int j = 0; j < NT; j++) {
-                                if (8 * j < rows) {
-                                    int d[MT][4];
+                                int d[4];
 #pragma unroll
-                                    for (int m = 0; m < MT; m++) d[m][0] = d[m][1] = d[m][2] = d[m][3] = Q4_MAGIC;
+                                for (int st = 0; st < GS / 32; st++) {
+                                    const uint2 b = *reinterpret_cast<const uint2 *>(xl + (8 * j + g) * Q4R_XROW + (c * GC + gc) * GS + 32 * st + 8 * t);
+                                    if (st == 0) mma_s8_first(d, A[st], b.x, b.y, Q4_MAGIC);
+                                    else mma_s8(d, A[st], b.x, b.y);
+                                }
+                                const float2 x = *reinterpret_cast<const float2 *>(xsm + (c * GC + gc) * R + 8 * j + 2 * t);
 #pragma unroll
-                                    for (int st = 0; st < GS / 32; st++) {
-                                        const uint2 b = __ldg(reinterpret_cast<const uint2 *>(xr[j] + grp * GS + 32 * st));
-#pragma unroll
-                                        for (int m = 0; m < MT; m++) mma_s8(d[m], A[m][st], b.x, b.y);
-                                    }
-                                    const float *xs = a.xs + (size_t)row0 * G + grp;
-                                    const float x0 = __ldg(xs + (size_t)min(8 * j + 2 * t, rows - 1) * G), x1 = __ldg(xs + (size_t)min(8 * j + 2 * t + 1, rows - 1) * G);
-#pragma unroll
-                                    for (int m = 0; m < MT; m++) {
-                                        const float o0 = -Q4_MAGIC_F * ws[m][0], o1 = -Q4_MAGIC_F * ws[m][1];
-                                        p[m][j][0] = fmaf(fmaf(__int_as_float(d[m][0]), ws[m][0], o0), x0, p[m][j][0]);
-                                        p[m][j][1] = fmaf(fmaf(__int_as_float(d[m][1]), ws[m][0], o0), x1, p[m][j][1]);
-                                        p[m][j][2] = fmaf(fmaf(__int_as_float(d[m][2]), ws[m][1], o1), x0, p[m][j][2]);
-                                        p[m][j][3] = fmaf(fmaf(__int_as_float(d[m][3]), ws[m][1], o1), x1, p[m][j][3]);
-                                    }
+                                for (int h = 0; h < 2; h++) {
+                                    p[m][j][2 * h] = fmaf(fmaf(__int_as_float(d[2 * h]), wf[h], of[h]), x.x, p[m][j][2 * h]);
+                                    p[m][j][2 * h + 1] = fmaf(fmaf(__int_as_float(d[2 * h + 1]), wf[h], of[h]), x.y, p[m][j][2 * h + 1]);
                                 }
                             }
                         }
                     }
+                    if (m + 1 < J) fetch(a.up, 4 * sl + c, c);
+                    else if constexpr (MULTI) fetch(a.w, 4 * (sl + NW) + c, c);
                 }
-                fetch(4 * (sl + NW) + c, c);
             }
+            __syncwarp();  // (the partial sums go where the levels were)
         }
-        if (s0 > 0) __syncthreads();  // the last round's partial sums have been read
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int m = 0; m < J; m++)
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                float *o = red + ((size_t)w * R + 8 * j + 2 * t) * FS + 16 * m + g;
-                o[0] = p[m][j][0];
-                o[FS] = p[m][j][1];
-                o[8] = p[m][j][2];
-                o[FS + 8] = p[m][j][3];
-            }
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float *o = red(w) + (8 * j + 2 * t) * FS + 16 * m + 8 * h + g;
+                    o[0] = p[m][j][2 * h];
+                    o[FS] = p[m][j][2 * h + 1];
+                }
         __syncthreads();
         const int nw = min(NW, W.slices - s0);
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(tot) / 4); i++) {
+        for (int i = 0; i < OWN; i++) {
             const int e = i * blockDim.x + threadIdx.x;
             if (e < R * FT)
                 for (int u = 0; u < nw; u += 2) {
-                    const float *o = red + ((size_t)u * R + e / FT) * FS + e % FT;
-                    tot[i] += u + 1 < nw ? o[0] + o[R * FS] : o[0];
+                    const int at = e / FT * FS + e % FT;
+                    tot[i] += u + 1 < nw ? red(u)[at] + red(u + 1)[at] : red(u)[at];
                 }
         }
     }
     if constexpr (!GATED) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(tot) / 4); i++) {
+        for (int i = 0; i < OWN; i++) {
             const int e = i * blockDim.x + threadIdx.x, r = e / FT;
             const int f = blockIdx.x * FT + e % FT;
-            if (e < R * FT && r < rows && f < W.n) a.out[(size_t)(row0 + r) * W.n + f] = tot[i];
+            if (e < R * FT && r < rows && f < W.n) a.out[(size_t)(row0 + r) * W.n + f] = tot[i] * 0.0625f;
         }
     } else {
         // the two products of an output are in different threads: through shared memory
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(tot) / 4); i++) {
+        for (int i = 0; i < OWN; i++) {
             const int e = i * blockDim.x + threadIdx.x;
-            if (e < R * FT) red[(size_t)(e / FT) * FS + e % FT] = tot[i];
+            if (e < R * FT) red(0)[e / FT * FS + e % FT] = tot[i] * 0.0625f;
         }
         __syncthreads();
-        float *h = red + R * FS, *top = h + R * 16;  // [R][16], [R]  (behind the sums: NW >= 2)
+        float *sum = red(0), *h = sum + R * FS, *top = h + R * 16;  // [R][FS], [R][16], [R]
         for (int e = threadIdx.x; e < R * 16; e += blockDim.x) {
             const int r = e >> 4, fo = e & 15, f = blockIdx.x * 16 + fo;
-            const float v = q4_silu_mul(red[r * FS + fo], red[r * FS + 16 + fo]);
+            const float v = q4_silu_mul(sum[r * FS + fo], sum[r * FS + 16 + fo]);
             if (a.out && r < rows && f < W.n) a.out[(size_t)(row0 + r) * W.n + f] = v;
             if (a.hq) {
                 float m = fabsf(v);
@@ -298,17 +331,17 @@ __global__ void __launch_bounds__(256) q4_rows_kernel(const Q4Args a) {
     }
 }
 
-template <int GS, int MT, int NT, bool GATED>
+template <int GS, int NT, bool GATED>
 cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
     const int NW = a.w.slices >= 8 ? 8 : 4;  // at least four warps own the outputs of the CTA
-    const size_t smem = (size_t)NW * 8 * NT * (16 * MT + 4) * sizeof(float);
-    auto kern = q4_rows_kernel<GS, MT, NT, GATED>;
+    const size_t smem = (size_t)NW * q4r_warp_bytes(GS, NT);
+    auto kern = a.w.slices > NW ? q4_rows_kernel<GS, NT, GATED, true> : q4_rows_kernel<GS, NT, GATED, false>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(GATED ? a.w.tiles : (a.w.tiles + MT - 1) / MT, (a.rows + 8 * NT - 1) / (8 * NT));
+    cfg.gridDim = dim3(a.w.tiles, (a.rows + 8 * NT - 1) / (8 * NT));
     cfg.blockDim = dim3(32 * NW);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -361,20 +394,15 @@ __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
-// Two adjacent rows of one output, as the halves of 64-bit registers (float2 values would be taken apart and put together again by moves):
-// p += round(D ws) xs for both rows, from the int32 sums d0, d1 (16 D); w2 = ws / 16 twice, o2 = -Q4_MAGIC_F w2.  The offset goes in by one
-// logic operation, (d & 0x7fffff) ^ 0x4B400000 (the sums fit 23 bits; flipping their sign bit adds 2^22): additions would be put on the pipe that
-// the multiply-adds need (630 against 530 clocks per 128 x 128 group in isolation).
+// Two adjacent rows of one output, as the halves of 64-bit registers (float2 values would be taken apart and put together again by moves)
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
     return r;
 }
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
+// p += round(16 D ws) xs for both rows, from the int32 sums d0, d1 (16 D); w2 = ws twice, o2 = -Q4_MAGIC_F w2.  The offset goes in by one
+// logic operation, (d & 0x7fffff) ^ 0x4B400000 (the sums fit 23 bits; flipping their sign bit adds 2^22): additions would be put on the pipe that
+// the multiply-adds need (630 against 530 clocks per 128 x 128 group in isolation).
 __device__ __forceinline__ void q4_add2(uint64_t &p, uint32_t d0, uint32_t d1, uint64_t w2, uint64_t o2, uint64_t x2) {
     asm("{\n.reg .b32 a, b;\n.reg .b64 t;\nlop3.b32 a, %1, %6, %7, 0x6a;\nlop3.b32 b, %2, %6, %7, 0x6a;\nmov.b64 t, {a, b};\nfma.rn.f32x2 t, t, %3, %4;\nfma.rn.f32x2 %0, t, %5, %0;\n}"
         : "+l"(p)
@@ -457,7 +485,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
         const int sl0 = chunk0 / 4, sl1 = (chunk1 + 3) / 4;
         // The scales of a slice, a slice ahead: loaded into registers (from clamped addresses, so that nothing waits for the loads before
         // they are stored) and stored to shared memory when the slice before is done.  Rows: element e = (row e / PER, group e % PER);
-        // outputs: four groups of one output per thread, times 1 / 16 (the levels are in the upper halves of their bytes).
+        // outputs: four groups of one output per thread.
         constexpr int XW = (128 * (PER / 4) + 32 * DW - 1) / (32 * DW), WT = 32 * DW / (PER / 4);
         float xn[XE];
         uint2 wn[XW];
@@ -488,7 +516,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
                 if (wf + WT * i < 128) {
                     const float2 lo = __half22float2(*reinterpret_cast<__half2 *>(&wn[i].x)), hi = __half22float2(*reinterpret_cast<__half2 *>(&wn[i].y));
                     float *o = wss + (slot * PER + wp) * 128 + wf + WT * i;
-                    o[0] = lo.x * 0.0625f, o[128] = lo.y * 0.0625f, o[256] = hi.x * 0.0625f, o[384] = hi.y * 0.0625f;
+                    o[0] = lo.x, o[128] = lo.y, o[256] = hi.x, o[384] = hi.y;
                 }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * DW) : "memory");
         };
@@ -650,10 +678,10 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     const int pairs = (W.chunks + 7) / 8;
     const uint32_t prank = (uint32_t)py * C;
     auto total = [&](int r, int f) {
-        if (C == 1) return sums[r * Q4T_FS + f];
+        if (C == 1) return sums[r * Q4T_FS + f] * 0.0625f;
         float t = 0.0f;
         for (int q = 0; q < pairs; q++) t += ld_cluster(sums + ((size_t)(q % np) * RT + r) * Q4T_FS + f, prank + q / np);
-        return t;
+        return t * 0.0625f;
     };
     if constexpr (!GATED) {
         for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32)
@@ -738,8 +766,9 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
     return cudaLaunchKernelEx(&cfg, kern, a, map, lst, np, C, P, err);
 }
 
-// Which rows per tile and how many CTAs along the inputs: the least estimated time, in clocks.  A group costs a CTA its drain (measured:
-// q4t_group) and a CTA costs its start and end; CTAs run one per SM, in waves.
+// Rows per tile and CTAs along the inputs with the least estimated time, in clocks.  CTAs run one per SM, in waves; a CTA costs 6,000 to start
+// and end (2,500 more in a cluster) and a chunk of 128 inputs a part for its stage and a part per group that is drained, as measured:
+// 32 rows 750 + 190, 64 rows 700 + 500, 128 rows 800 + 1,000.
 struct Q4Plan {
     int rt, c;
 };
@@ -748,30 +777,34 @@ inline Q4Plan q4_plan(const Q4Args &a, bool gated, int n_sm) {
     Q4Plan best = {128, 1};
     double least = 1e300;
     for (int rt = 32; rt <= 128; rt *= 2) {
-        const double group = rt == 128 ? 330.0 : rt == 64 ? 180.0 : 120.0;
+        const double chunk = rt == 128 ? 800.0 + 1000.0 * (Q4_CHUNK / a.w.gs) : rt == 64 ? 700.0 + 500.0 * (Q4_CHUNK / a.w.gs) : 750.0 + 190.0 * (Q4_CHUNK / a.w.gs);
         for (int c = 1; c * P <= 8 && c <= pairs; c++) {
             const int np = (pairs + c - 1) / c;
             if ((pairs + np - 1) / np != c) continue;
             if (1024 + q4t_scales(a.w.gs, rt) + q4t_sums(rt) * (c > 1 ? np : 1) + 2 * q4t_stage(rt) > 226 * 1024) continue;
             const long long ctas = (long long)c * tiles * ((a.rows + rt - 1) / rt), slots = n_sm / (c * P) * (c * P);
-            const double time = (double)((ctas + slots - 1) / slots) * (3000.0 + (c > 1 ? 1500.0 : 0.0) + (double)np * (Q4_PAIR / a.w.gs) * group);
+            const double time = (double)((ctas + slots - 1) / slots) * (6000.0 + (c > 1 ? 2500.0 : 0.0) + (double)np * (Q4_PAIR / Q4_CHUNK) * chunk);
             if (time < least) least = time, best = {rt, c};
         }
     }
     return best;
 }
 
+// Up to this many rows the kernel for few rows is the faster one (blocks of 16 rows; measured with groups of 64: 48 x 6144 x 4096 14.6 against
+// 20.3 us, 64 x 6144 x 4096 19.2 against 20.3 us, 64 x 4096 x 12288 38.3 against 31.8 us).
+constexpr int Q4_FEW = 56;
+
 template <int GS>
 cudaError_t launch_q4_gs(const Q4Args &a, bool gated, int n_sm, Q4EncodeFn enc, int *err, cudaStream_t stream) {
-#define Q4_BY_ROWS(MT_, GATED_)                                           \
-    if (a.rows <= 8) return launch_q4_rows<GS, MT_, 1, GATED_>(a, stream); \
-    if (a.rows <= 16) return launch_q4_rows<GS, MT_, 2, GATED_>(a, stream); \
-    const Q4Plan plan = q4_plan(a, GATED_, n_sm);                          \
+#define Q4_BY_ROWS(GATED_)                                                                  \
+    if (a.rows <= 8) return launch_q4_rows<GS, 1, GATED_>(a, stream);                       \
+    if (a.rows <= Q4_FEW) return launch_q4_rows<GS, 2, GATED_>(a, stream);                  \
+    const Q4Plan plan = q4_plan(a, GATED_, n_sm);                                           \
     if (plan.rt == 32) return launch_q4_tiles<GS, 32, GATED_>(a, plan.c, enc, err, stream); \
     if (plan.rt == 64) return launch_q4_tiles<GS, 64, GATED_>(a, plan.c, enc, err, stream); \
     return launch_q4_tiles<GS, 128, GATED_>(a, plan.c, enc, err, stream)
-    if (gated) { Q4_BY_ROWS(2, true); }
-    Q4_BY_ROWS(1, false);
+    if (gated) { Q4_BY_ROWS(true); }
+    Q4_BY_ROWS(false);
 #undef Q4_BY_ROWS
 }
 
