@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256, NT == 1 && GS >= 64 ? 3 : NT <= 2 ? 2 : 1
                     uint32_t at;
                     float v;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(top + r)), "r"(q));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
                     m = fmaxf(m, v);
                 }
                 if (r < rows) {
@@ -391,7 +391,7 @@ __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
     uint32_t at;
     float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
     return v;
 }
 // Two adjacent rows of one output, as the halves of 64-bit registers (float2 values would be taken apart and put together again by moves)
@@ -677,29 +677,46 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     const int share = (RT + C - 1) / C, r0 = kc * share, r1 = min(min(r0 + share, RT), a.rows - row0);
     const int pairs = (W.chunks + 7) / 8;
     const uint32_t prank = (uint32_t)py * C;
-    auto total = [&](int r, int f) {
-        if (C == 1) return sums[r * Q4T_FS + f] * 0.0625f;
-        float t = 0.0f;
-        for (int q = 0; q < pairs; q++) t += ld_cluster(sums + ((size_t)(q % np) * RT + r) * Q4T_FS + f, prank + q / np);
-        return t * 0.0625f;
+    // outputs f, f + 32, f + 64, f + 96 of row r: the pairs' sums in order (the four sums' remote loads overlap)
+    auto totals = [&](int r, int f, float *t) {
+        if (C == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[i] = sums[r * Q4T_FS + f + 32 * i] * 0.0625f;
+            return;
+        }
+        t[0] = t[1] = t[2] = t[3] = 0.0f;
+#pragma unroll 2
+        for (int q = 0; q < pairs; q++) {
+            const float *o = sums + ((size_t)(q % np) * RT + r) * Q4T_FS + f;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = ld_cluster(o + 32 * i, prank + q / np);
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[i] += v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] *= 0.0625f;
     };
     if constexpr (!GATED) {
-        for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32)
+        for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32) {
+            float v[4];
+            totals(r, lane, v);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int f = ft * 128 + 32 * i + lane;
-                const float v = total(r, 32 * i + lane);
-                if (f < W.n) a.out[(size_t)(row0 + r) * W.n + f] = v;
+                if (f < W.n) a.out[(size_t)(row0 + r) * W.n + f] = v[i];
             }
+        }
     } else {
         for (int pass = a.hq && GS == 128 ? 0 : 1; pass < 2; pass++) {
             if (pass == 1 && a.hq && GS == 128) cluster_sync_all();  // the two CTAs of a group's halves have their maxima
             for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32) {
-                float v[2];
+                float s[4], v[2];  // gate, gate, up, up
                 uint32_t m[2];
+                totals(r, lane, s);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    v[i] = q4_silu_mul(total(r, 32 * i + lane), total(r, 64 + 32 * i + lane));
+                    v[i] = q4_silu_mul(s[i], s[2 + i]);
                     m[i] = a.hq ? __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(v[i]), 0.0f))) : 0u;  // (a NaN counts as 0)
                 }
                 if (GS >= 64) m[0] = m[1] = max(m[0], m[1]);
@@ -790,15 +807,17 @@ inline Q4Plan q4_plan(const Q4Args &a, bool gated, int n_sm) {
     return best;
 }
 
-// Up to this many rows the kernel for few rows is the faster one (blocks of 16 rows; measured with groups of 64: 48 x 6144 x 4096 14.6 against
+// Up to this many rows the kernel for few rows is the faster one (in blocks of 8 or 16 rows, a block of 16 costs 1.75 blocks of 8; measured with groups of 64: 48 x 6144 x 4096 14.6 against
 // 20.3 us, 64 x 6144 x 4096 19.2 against 20.3 us, 64 x 4096 x 12288 38.3 against 31.8 us).
 constexpr int Q4_FEW = 56;
 
 template <int GS>
 cudaError_t launch_q4_gs(const Q4Args &a, bool gated, int n_sm, Q4EncodeFn enc, int *err, cudaStream_t stream) {
 #define Q4_BY_ROWS(GATED_)                                                                  \
-    if (a.rows <= 8) return launch_q4_rows<GS, 1, GATED_>(a, stream);                       \
-    if (a.rows <= Q4_FEW) return launch_q4_rows<GS, 2, GATED_>(a, stream);                  \
+    if (a.rows <= Q4_FEW) {                                                                 \
+        if (7 * ((a.rows + 15) / 16) > 4 * ((a.rows + 7) / 8)) return launch_q4_rows<GS, 1, GATED_>(a, stream); \
+        return launch_q4_rows<GS, 2, GATED_>(a, stream);                                    \
+    }                                                                                       \
     const Q4Plan plan = q4_plan(a, GATED_, n_sm);                                           \
     if (plan.rt == 32) return launch_q4_tiles<GS, 32, GATED_>(a, plan.c, enc, err, stream); \
     if (plan.rt == 64) return launch_q4_tiles<GS, 64, GATED_>(a, plan.c, enc, err, stream); \
