@@ -374,11 +374,27 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
 // in its shared memory and each CTA adds up its share of the rows in the one order, reading from the others'.
 constexpr int Q4T_DRAIN = 8, Q4T_FS = 132, Q4T_BAND = 12;
 __host__ __device__ constexpr int q4t_unpack(int rt) { return rt == 128 ? 4 : 8; }  // unpack warps
-__host__ __device__ constexpr int q4t_threads(int rt) { return 32 * (Q4T_DRAIN + q4t_unpack(rt) + 1); }
+__host__ __device__ constexpr int q4t_threads(int rt) { return 32 * (Q4T_DRAIN + q4t_unpack(rt) + 4); }  // (the MMA warp's warpgroup has three idle warps)
 __host__ __device__ constexpr int q4t_stage(int rt) { return 16384 + rt * 128; }
 __host__ __device__ constexpr int q4t_scales(int gs, int rt) { return 2 * (Q4_SLICE / gs) * (rt + 128) * 4; }  // two slices' scales of the rows and of the outputs
 __host__ __device__ constexpr int q4t_sums(int rt) { return rt * Q4T_FS * 4; }  // one pair's sums [RT][132]
 
+// The registers of a warpgroup: the drain gets what the others do not need.  Per SM: 32 rows or 64 a tile, 20 warps of 96 at launch: 8 x 128 + 8 x 88 +
+// 4 x 40 = 1,888 of 1,920; 128 rows, 16 warps of 128: 8 x 184 + 4 x 96 + 4 x 40 = 2,016 of 2,048 (times 32).
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// whether a phase is complete, without waiting
+__device__ __forceinline__ bool mbar_try_now(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
 __device__ __forceinline__ void ldg_stream8(const void *p, uint32_t *r) {
     asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -474,12 +490,14 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     pdl_wait();
 
     if (warp < DW) {
+        setmaxnreg_inc<RT == 128 ? 184 : 128>();
         // ---- drain: the warp's 32 outputs x RC rows in accumulator-fragment layout, output 8 k + lane / 4, rows col0 + 8 i + 2 (lane % 4) + 0, 1
         const int quad = warp & 3, col0 = (warp >> 2) * RC, g4 = lane >> 2, t2 = 2 * (lane & 3);
         const uint32_t mine = tbase + ((uint32_t)(quad * 32) << 16) + col0;
         constexpr int NI = RC / 8;
         uint64_t p[4][NI];  // row pairs
-        bool ok = true;
+        bool ready = false;  // the next D buffer is known to be complete
+        const uint64_t minus_magic = pack2(-Q4_MAGIC_F, -Q4_MAGIC_F);
         int buf = 0;
         uint32_t ph = 0;  // the next D buffer and the phase of its barrier
         const int sl0 = chunk0 / 4, sl1 = (chunk1 + 3) / 4;
@@ -532,23 +550,28 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
             const float *xsl = xss + slot * PER * RT + col0 + t2, *wsl = wss + slot * PER * 128 + quad * 32 + g4;
 #pragma unroll 1
             for (int b = 0; b < bufs; b++) {
-                if (ok) ok = mbar_wait_bounded_quiet(dfull + buf, ph, err, 82);
-                ok = __all_sync(0xffffffffu, ok);
+                // (asked for ahead: the answer takes ~140 clocks.  After a wait that ran out the loop goes on, with nothing but numbers at stake)
+                if (!ready) mbar_wait_bounded_quiet(dfull + buf, ph, err, 82);
+                __syncwarp();
                 tc_fence_after();
+                const uint32_t dbuf = mine + buf * 128;
+                uint64_t *const free_bar = dempty + buf;
+                buf ^= 1, ph ^= buf == 0;
 #pragma unroll
                 for (int g = 0; g < GB; g++) {
                     const int at = b * GB + g;
                     uint64_t w2[4], o2[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const float w = wsl[at * 128 + 8 * k], o = -Q4_MAGIC_F * w;
-                        w2[k] = pack2(w, w), o2[k] = pack2(o, o);
+                        const float w = wsl[at * 128 + 8 * k];
+                        w2[k] = pack2(w, w);
+                        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o2[k]) : "l"(w2[k]), "l"(minus_magic));
                     }
 #pragma unroll
                     for (int c = 0; c < RC; c += UC) {
                         uint32_t r[2][4 * NU];
 #pragma unroll
-                        for (int h = 0; h < 2; h++) tmem_ld_frag<NU>(mine + ((uint32_t)(16 * h) << 16) + buf * 128 + g * RT + c, r[h]);
+                        for (int h = 0; h < 2; h++) tmem_ld_frag<NU>(dbuf + ((uint32_t)(16 * h) << 16) + g * RT + c, r[h]);
                         uint64_t x2[NU];
 #pragma unroll
                         for (int i = 0; i < NU; i++) x2[i] = *reinterpret_cast<const uint64_t *>(xsl + at * RT + c + 8 * i);
@@ -556,7 +579,8 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
                         if (g == GB - 1 && c + UC == RC) {
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(dempty + buf);
+                            if (lane == 0) mbar_arrive(free_bar);
+                            ready = mbar_try_now(dfull + buf, ph);
                         }
 #pragma unroll
                         for (int i = 0; i < NU; i++)
@@ -564,7 +588,6 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
                             for (int k = 0; k < 4; k++) q4_add2(p[k][c / 8 + i], r[k >> 1][4 * i + 2 * (k & 1)], r[k >> 1][4 * i + 2 * (k & 1) + 1], w2[k], o2[k], x2[i]);
                     }
                 }
-                buf ^= 1, ph ^= buf == 0;
             }
             // the end of the slice: hold p, or add it to the slice before and keep the pair (C > 1) or add it to the total
             constexpr int NE = NI < 4 ? NI : 4;  // pieces of 8 NE rows
@@ -604,6 +627,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
             if (sl + 1 < sl1) put_scales(sl + 1, slot ^ 1);
         }
     } else if (u < UW) {
+        setmaxnreg_dec<RT == 128 ? 96 : 88>();
         bool ok = true;
         const int f = lane & 15, h = lane >> 4;
         uint8_t *out[4];  // the lane's four 16-byte places in the first tile of its part
@@ -637,7 +661,9 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
         }
         if (lane == 0 && *reinterpret_cast<volatile int *>(err) != 0)  // a wait ran out: the copies in flight get a bounded time to land
             for (int i = 0; i < (1 << lst); i++) mbar_drain(full + i, 0), mbar_drain(full + i, 1);
-    } else if (elect_one()) {
+    } else {
+        setmaxnreg_dec<40>();
+        if (u == UW && elect_one()) {
         // ---- MMA issue
         constexpr uint32_t idesc = umma_idesc_i8(128, RT, 0, 0, 1, 1);
         const uint32_t sbase = smem_u32(sm);
@@ -666,12 +692,18 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
         }
         umma_commit(&done);
         mbar_drain(&done, 0);  // (no MMA and no arrival of one is in flight when the CTA ends)
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == DW + UW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512));
     if (C > 1) cluster_sync_all();  // (the clusters of 128-wide groups and C = 1 have nothing to read here yet)
+    if (warp >= DW) {  // the other roles have only the cluster's barriers left
+        if (GATED && a.hq && GS == 128) cluster_sync_all();
+        if (C > 1 || P > 1) cluster_sync_all();
+        return;
+    }
 
     // ---- the totals of this CTA's share of the rows, a warp per row, lanes along the outputs
     const int share = (RT + C - 1) / C, r0 = kc * share, r1 = min(min(r0 + share, RT), a.rows - row0);
@@ -698,7 +730,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
         for (int i = 0; i < 4; i++) t[i] *= 0.0625f;
     };
     if constexpr (!GATED) {
-        for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32) {
+        for (int r = r0 + warp; r < r1; r += DW) {
             float v[4];
             totals(r, lane, v);
 #pragma unroll
@@ -710,7 +742,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     } else {
         for (int pass = a.hq && GS == 128 ? 0 : 1; pass < 2; pass++) {
             if (pass == 1 && a.hq && GS == 128) cluster_sync_all();  // the two CTAs of a group's halves have their maxima
-            for (int r = r0 + warp; r < r1; r += q4t_threads(RT) / 32) {
+            for (int r = r0 + warp; r < r1; r += DW) {
                 float s[4], v[2];  // gate, gate, up, up
                 uint32_t m[2];
                 totals(r, lane, s);
