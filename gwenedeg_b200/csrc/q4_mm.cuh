@@ -103,7 +103,7 @@ __device__ __forceinline__ void mma_s8_first(int *d, const uint32_t *a, uint32_t
 // An int32 sum S plus the bits of 1.5 2^23 are the bits of the float 1.5 2^23 + S, exactly, while |S| < 2^22 (here S = 16 D, as the levels
 // sit in the upper halves of their bytes: |S| <= 16 . 128 . 8 . 128 = 2^21).  With M = 1.5 2^23:  fma(M + S, ws, -M ws) = round(S ws): M ws is
 // exact (ws has 11 significant bits), so one multiply-add converts, removes the offset and applies the weight's scale, with the one rounding
-// of the product.  The factor 16 is carried to the end, where the total is multiplied by 1 / 16 (both exact).
+// of the product.  The factor 16 is carried to the end, where the total is multiplied by 1 / 16 (both exact while 16 |y| is below 2^128).
 constexpr int Q4_MAGIC = 0x4B400000;
 constexpr float Q4_MAGIC_F = 12582912.0f;
 
@@ -368,8 +368,12 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
 //   4 or 8 warps    unpack: a quarter of a chunk each, 1 KB of a tile per load, straight from the layout (registers, four steps ahead), to int8 rows of 128 inputs with
 //                   the 128-byte swizzle (K-major A operand); a chunk's first step also asks for the rows' levels by TMA (K-major B operand)
 //   one warp        issues the MMAs into two D buffers in turn, of as many groups as fill 128 columns (up to a chunk's)
-// What bounds it is the drain: per D value an addition, two multiply-adds and its part of the loads and waits, against 4,096 or more products per
-// clock in the tensor core; 16 warps, because two per scheduler left it waiting for TMEM loads most of the time.
+// What bounds it is the drain: per D value one logic operation, two multiply-adds and its part of the loads, about 1,900 warp instructions per 128 x 128
+// group of which 512 are packed multiply-adds on a pipe that takes one every two clocks, and two drain warps per scheduler that issue half
+// of the time: 960 clocks per group, against 128 for its products (tensor pipe 8 % busy).  Measured: 2000 x 6144 x 4096 268 us with groups of 64, 512 x 4096
+// x 12288 81 us with groups of 128 (633 TOP/s).  16 drain warps, TMEM loads a half buffer ahead, and three buffers changed nothing;
+// integer conversions instead of the offset cost 15 %, additions of the offset (which the compiler puts on the multiply-add pipe) 5 %, four
+// unpack warps instead of eight at 32 and 64 rows 40 %.
 // With few tiles the inputs are split over the C CTAs of a cluster at multiples of 1,024: every CTA leaves the sums of its pairs of slices
 // in its shared memory and each CTA adds up its share of the rows in the one order, reading from the others'.
 constexpr int Q4T_DRAIN = 8, Q4T_FS = 132, Q4T_BAND = 12;
@@ -664,34 +668,34 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     } else {
         setmaxnreg_dec<40>();
         if (u == UW && elect_one()) {
-        // ---- MMA issue
-        constexpr uint32_t idesc = umma_idesc_i8(128, RT, 0, 0, 1, 1);
-        const uint32_t sbase = smem_u32(sm);
-        int buf = 0;
-        uint32_t ph = 1;  // the phase of the D buffer's barrier before its last release (the first round does not wait)
-        bool ok = true;
-        for (int chunk = chunk0; chunk < chunk1 && ok; chunk++) {
-            const int rel = chunk - chunk0, st = rel & ((1 << lst) - 1);
-            ok = mbar_wait_bounded_quiet(full + st, (uint32_t)(rel >> lst) & 1u, err, 85);
-            const uint32_t A = sbase + st * q4t_stage(RT), B = A + 16384;
+            // ---- MMA issue
+            constexpr uint32_t idesc = umma_idesc_i8(128, RT, 0, 0, 1, 1);
+            const uint32_t sbase = smem_u32(sm);
+            int buf = 0;
+            uint32_t ph = 1;  // the phase of the D buffer's barrier before its last release (the first round does not wait)
+            bool ok = true;
+            for (int chunk = chunk0; chunk < chunk1 && ok; chunk++) {
+                const int rel = chunk - chunk0, st = rel & ((1 << lst) - 1);
+                ok = mbar_wait_bounded_quiet(full + st, (uint32_t)(rel >> lst) & 1u, err, 85);
+                const uint32_t A = sbase + st * q4t_stage(RT), B = A + 16384;
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                if (ok && (rel * NB + b >= 2)) ok = mbar_wait_bounded_quiet(dempty + buf, ph, err, 86);
-                if (ok) {
-                    tc_fence_after();
+                for (int b = 0; b < NB; b++) {
+                    if (ok && (rel * NB + b >= 2)) ok = mbar_wait_bounded_quiet(dempty + buf, ph, err, 86);
+                    if (ok) {
+                        tc_fence_after();
 #pragma unroll
-                    for (int s = 0; s < GB * GS / 32; s++) {
-                        const int at = b * GB * GS + 32 * s;
-                        umma_i8(tbase + buf * 128 + s / (GS / 32) * RT, umma_desc(A + at, 16, 1024, 2), umma_desc(B + at, 16, 1024, 2), idesc, s % (GS / 32) > 0);
+                        for (int s = 0; s < GB * GS / 32; s++) {
+                            const int at = b * GB * GS + 32 * s;
+                            umma_i8(tbase + buf * 128 + s / (GS / 32) * RT, umma_desc(A + at, 16, 1024, 2), umma_desc(B + at, 16, 1024, 2), idesc, s % (GS / 32) > 0);
+                        }
+                        umma_commit(dfull + buf);
+                        buf ^= 1, ph ^= buf == 0;
                     }
-                    umma_commit(dfull + buf);
-                    buf ^= 1, ph ^= buf == 0;
                 }
+                umma_commit(empty + st);
             }
-            umma_commit(empty + st);
-        }
-        umma_commit(&done);
-        mbar_drain(&done, 0);  // (no MMA and no arrival of one is in flight when the CTA ends)
+            umma_commit(&done);
+            mbar_drain(&done, 0);  // (no MMA and no arrival of one is in flight when the CTA ends)
         }
     }
     __syncwarp();
@@ -817,7 +821,7 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
 
 // Rows per tile and CTAs along the inputs with the least estimated time, in clocks.  CTAs run one per SM, in waves; a CTA costs 6,000 to start
 // and end (2,500 more in a cluster) and a chunk of 128 inputs a part for its stage and a part per group that is drained, as measured:
-// 32 rows 750 + 190, 64 rows 700 + 500, 128 rows 800 + 1,000.
+// 32 rows 750 + 190, 64 rows 700 + 500, 128 rows 650 + 960.
 struct Q4Plan {
     int rt, c;
 };
@@ -826,7 +830,7 @@ inline Q4Plan q4_plan(const Q4Args &a, bool gated, int n_sm) {
     Q4Plan best = {128, 1};
     double least = 1e300;
     for (int rt = 32; rt <= 128; rt *= 2) {
-        const double chunk = rt == 128 ? 800.0 + 1000.0 * (Q4_CHUNK / a.w.gs) : rt == 64 ? 700.0 + 500.0 * (Q4_CHUNK / a.w.gs) : 750.0 + 190.0 * (Q4_CHUNK / a.w.gs);
+        const double chunk = rt == 128 ? 650.0 + 960.0 * (Q4_CHUNK / a.w.gs) : rt == 64 ? 700.0 + 500.0 * (Q4_CHUNK / a.w.gs) : 750.0 + 190.0 * (Q4_CHUNK / a.w.gs);
         for (int c = 1; c * P <= 8 && c <= pairs; c++) {
             const int np = (pairs + c - 1) / c;
             if ((pairs + np - 1) / np != c) continue;

@@ -284,6 +284,81 @@ def test_gated_rows_do_not_depend_on_the_other_rows(ctx, dev):
         assert np.array_equal(dev.get(hs, (rows, n // gs)), all_s[r0:r0 + rows])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,gs", [(256, 4224, 128), (160, 2080, 32), (192, 8256, 64)])
+def test_gated_rows_in_8_bits_over_every_kernel(ctx, dev, n, k, gs):
+    """Few rows, many rows, inputs split over a cluster or not, groups inside a tile and across two: the same bits for the same row; a row
+    whose scale is no number stays alone."""
+    rng = np.random.default_rng(k + gs)
+    most = 300
+    gl, gsc = matrix(rng, n, k, gs)
+    ul, usc = matrix(rng, n, k, gs)
+    xq, xs = rows8(rng, most, k, gs)
+    xs *= np.float32(0.3)
+    xs[2, 1] = np.nan
+    gate, up = ctx.q4_new(packed(gl), gsc, gs), ctx.q4_new(packed(ul), usc, gs)
+    q, s = dev.put(xq), dev.put(xs)
+    h, hq, hs = dev.room((most, n), np.float32), dev.room((most, n), np.int8), dev.room((most, n // gs), np.float32)
+    first = None
+    for rows in (1, 3, 8, 9, 24, 56, 57, 64, 65, 100, 128, 129, 200, most):
+        ctx.ffn_q4_dev(gate, up, rows, q, s, h, hq, hs)
+        got = dev.get(h, (rows, n)), dev.get(hq, (rows, n), np.int8), dev.get(hs, (rows, n // gs))
+        if rows == 3:
+            first = got
+            ok = [0, 1]
+            lev, top = quantised(got[0][ok], gs)
+            assert np.array_equal(got[1][ok], lev) and np.array_equal(got[2][ok], top * np.float32(1.0 / 127.0))
+            assert np.isnan(got[0][2]).all() and (got[1][2] == 0).all() and (got[2][2] == 0).all()
+        elif rows > 3:
+            for a, b in zip(got, first):
+                assert np.array_equal(a[:3].view(np.uint8), b.view(np.uint8)), rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,gs", [(1, 48, 20480, 64), (20, 48, 20480, 128), (70, 144, 20480, 32), (130, 144, 12320, 32), (57, 528, 3584, 64), (260, 1040, 1536, 128)])
+def test_long_inputs_and_ragged_tiles(ctx, dev, rows, n, k, gs):
+    rng = np.random.default_rng(rows + k)
+    lev, sc = matrix(rng, n, k, gs)
+    xq, xs = rows8(rng, rows, k, gs)
+    w = ctx.q4_new(packed(lev), sc, gs)
+    out = dev.room((rows, n), np.float32)
+    ctx.mm_q4_dev(w, rows, dev.put(xq), dev.put(xs), out)
+    want, tol = product(xq, xs, lev, sc, gs)
+    got = dev.get(out, (rows, n))
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_the_same_time():
+    """Two contexts, each on a stream of its own, with work of both in flight: the results are those of the calls made alone."""
+    import gwenedeg_b200 as gw
+    rng = np.random.default_rng(21)
+    n, k, gs = 640, 2176, 64
+    cs = [gw.Context(0, n_attn=1, n_heads=8, n_kv_heads=2, head_dim=128, max_rows=256) for _ in range(2)]
+    ds = [Dev(c) for c in cs]
+    lev, sc = matrix(rng, n, k, gs)
+    ms = [c.q4_new(packed(lev), sc, gs) for c in cs]
+    ins = [[rows8(rng, rows, k, gs) for rows in (1, 40, 200)] for _ in cs]
+    ptr = [[(d.put(q), d.put(s), d.room((q.shape[0], n), np.float32)) for q, s in i] for d, i in zip(ds, ins)]
+    alone = []
+    for c, d, m, pp, ii in zip(cs, ds, ms, ptr, ins):
+        for (q, s, o), (xq, _) in zip(pp, ii):
+            c.mm_q4_dev(m, xq.shape[0], q, s, o)
+            alone.append(d.get(o, (xq.shape[0], n)))
+    for _ in range(20):
+        for j in range(3):
+            for c, m, pp, ii in zip(cs, ms, ptr, ins):
+                c.mm_q4_dev(m, ii[j][0].shape[0], *pp[j])
+    at = 0
+    for d, pp, ii in zip(ds, ptr, ins):
+        for (q, s, o), (xq, _) in zip(pp, ii):
+            assert np.array_equal(d.get(o, (xq.shape[0], n)), alone[at])
+            at += 1
+    for d, c in zip(ds, cs):
+        d.free()
+        c.close()
+
+
 # ---- the norm ---------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,gs", [(1, 32, 32), (3, 96, 32), (2, 128, 128), (77, 2720, 32), (5, 4096, 64), (64, 4096, 128), (2, 8320, 64), (1, 32768, 128),
