@@ -128,9 +128,9 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src, bool valid
 constexpr int Q4R_XROW = Q4_SLICE + 32;  // bytes from row to row of a slice's levels
 __host__ __device__ constexpr int q4r_warp_bytes(int gs, int nt) { return 8 * nt * (Q4R_XROW + Q4_SLICE / gs * 4); }
 
-// MULTI: more slices than warps
-template <int GS, int NT, bool GATED, bool MULTI>
-__global__ void __launch_bounds__(256, NT == 1 && GS >= 64 ? 3 : NT <= 2 ? 2 : 1) q4_rows_kernel(const Q4Args a) {
+// MULTI: more slices than warps;  MOST: threads at most
+template <int GS, int NT, bool GATED, bool MULTI, int MOST>
+__global__ void __launch_bounds__(MOST, MOST > 256 ? 1 : NT == 1 && GS >= 64 ? 3 : NT <= 2 ? 2 : 1) q4_rows_kernel(const Q4Args a) {
     constexpr int GC = Q4_CHUNK / GS;        // groups per chunk
     constexpr int PER = Q4_SLICE / GS;       // groups per slice
     constexpr int J = GATED ? 2 : 1;         // matrices
@@ -333,9 +333,15 @@ __global__ void __launch_bounds__(256, NT == 1 && GS >= 64 ? 3 : NT <= 2 ? 2 : 1
 
 template <int GS, int NT, bool GATED>
 cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
-    const int NW = a.w.slices >= 8 ? 8 : 4;  // at least four warps own the outputs of the CTA
+    // A warp per slice up to 24 of them where the registers allow it (groups of 64 or 128, 8 rows), up to 8 else; at least four warps own the
+    // outputs of the CTA
+    constexpr bool WIDE = NT == 1 && GS >= 64;
+    const bool wide = WIDE && a.w.slices > 8 && a.w.slices <= 24;
+    const int NW = wide ? (a.w.slices + 1) / 2 * 2 : a.w.slices >= 8 ? 8 : 4;
     const size_t smem = (size_t)NW * q4r_warp_bytes(GS, NT);
-    auto kern = a.w.slices > NW ? q4_rows_kernel<GS, NT, GATED, true> : q4_rows_kernel<GS, NT, GATED, false>;
+    auto kern = a.w.slices > NW ? q4_rows_kernel<GS, NT, GATED, true, 256> : q4_rows_kernel<GS, NT, GATED, false, 256>;
+    if constexpr (WIDE)
+        if (wide) kern = q4_rows_kernel<GS, NT, GATED, false, 768>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
