@@ -1797,7 +1797,7 @@ int rq_cuda_dn_out_dev(RqCuda *c, int lin_layer, const float *rows, float *out) 
     return RQ_CUDA_OK;
 }
 
-// ---------------------------------------------------------------------------------------------------- the products around it
+// -------------------------------------------------------------------------------------- the products around the attention
 }  // extern "C"
 
 struct RqCudaQ4 {
@@ -1859,7 +1859,9 @@ void rq_cuda_q4_free(RqCudaQ4 *w) {
 size_t rq_cuda_q4_bytes(const RqCudaQ4 *w) { return w ? w->bytes : 0; }
 
 int rq_cuda_q4_new_dev(RqCuda *c, int n, int k, int gs, const unsigned char *levels, const unsigned short *scales, RqCudaQ4 **out) {
-    if (c && levels && scales && (((uintptr_t)levels & 3) || ((uintptr_t)scales & 1))) return fail(c, RQ_CUDA_ERR_ARG, "q4_new: levels must be 4-byte, scales 2-byte aligned");
+    if (out) *out = nullptr;
+    if (c && levels && scales && (((uintptr_t)levels & 3) || ((uintptr_t)scales & 1)))
+        return fail(c, RQ_CUDA_ERR_ARG, "q4_new: levels must be 4-byte, scales 2-byte aligned");
     int rc = q4_alloc(c, n, k, gs, levels, scales, out);
     if (rc) return rc;
     if ((rc = q4_fill(c, *out, levels, scales))) {
