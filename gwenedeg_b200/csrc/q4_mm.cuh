@@ -371,15 +371,16 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
 //   warps 0 .. 7    drain: a warp owns 32 outputs x RT / 2 rows in accumulator-fragment layout (4 outputs per thread: a scale read from
 //                   shared memory serves several values): p = fma(D ws, xs, p), packed over row pairs; the scales are staged by
 //                   these warps a slice ahead; the first slice of a pair rests in TMEM
-//   4 or 8 warps    unpack: a quarter of a chunk each, 1 KB of a tile per load, straight from the layout (registers, four steps ahead), to int8 rows of 128 inputs with
-//                   the 128-byte swizzle (K-major A operand); a chunk's first step also asks for the rows' levels by TMA (K-major B operand)
+//   4 or 8 warps    unpack: a quarter of a chunk each, 1 KB of a tile per load, straight from the layout (registers, four steps ahead), to
+//                   int8 rows of 128 inputs with the 128-byte swizzle (K-major A operand); the warp of a chunk's first quarter also asks
+//                   for the rows' levels by TMA (K-major B operand)
 //   one warp        issues the MMAs into two D buffers in turn, of as many groups as fill 128 columns (up to a chunk's)
-// What bounds it is the drain: per D value one logic operation, two multiply-adds and its part of the loads, about 1,900 warp instructions per 128 x 128
-// group of which 512 are packed multiply-adds on a pipe that takes one every two clocks, and two drain warps per scheduler that issue half
-// of the time: 960 clocks per group, against 128 for its products (tensor pipe 8 % busy).  Measured: 2000 x 6144 x 4096 268 us with groups of 64, 512 x 4096
-// x 12288 81 us with groups of 128 (633 TOP/s).  16 drain warps, TMEM loads a half buffer ahead, and three buffers changed nothing;
-// integer conversions instead of the offset cost 15 %, additions of the offset (which the compiler puts on the multiply-add pipe) 5 %, four
-// unpack warps instead of eight at 32 and 64 rows 40 %.
+// What bounds it is the drain: per D value one logic operation, two multiply-adds and its part of the loads, about 1,900 warp instructions per
+// 128 x 128 group, of which 512 are packed multiply-adds on a pipe that takes one every two clocks, and two drain warps per scheduler that
+// issue half of the time: 960 clocks per group, against 128 for its products (tensor pipe 10 % busy, 16 % with groups of 128).  Measured:
+// 2000 x 6144 x 4096 268 us with groups of 64, 512 x 4096 x 12288 81 us with groups of 128 (633 TOP/s).  16 drain warps, TMEM loads ahead of their
+// use, and three buffers brought nothing; integer conversions instead of the offset cost 15 %, additions of the offset (which the compiler
+// puts on the multiply-add pipe) 5 %, three unpack warps instead of eight at 32 and 64 rows 40 %.
 // With few tiles the inputs are split over the C CTAs of a cluster at multiples of 1,024: every CTA leaves the sums of its pairs of slices
 // in its shared memory and each CTA adds up its share of the rows in the one order, reading from the others'.
 constexpr int Q4T_DRAIN = 8, Q4T_FS = 132, Q4T_BAND = 12;
@@ -849,8 +850,8 @@ inline Q4Plan q4_plan(const Q4Args &a, bool gated, int n_sm) {
     return best;
 }
 
-// Up to this many rows the kernel for few rows is the faster one (in blocks of 8 or 16 rows, a block of 16 costs 1.75 blocks of 8; measured with groups of 64: 48 x 6144 x 4096 14.6 against
-// 20.3 us, 64 x 6144 x 4096 19.2 against 20.3 us, 64 x 4096 x 12288 38.3 against 31.8 us).
+// Up to this many rows the kernel for few rows is the faster one, in blocks of 8 or 16 rows (a block of 16 costs 1.75 blocks of 8).  Measured with
+// groups of 64: 48 x 6144 x 4096 14.3 against 20.3 us, 64 x 6144 x 4096 19.2 against 20.3 us, 64 x 4096 x 12288 38.3 against 30.5 us.
 constexpr int Q4_FEW = 56;
 
 template <int GS>

@@ -319,8 +319,8 @@ int rq_cuda_dn_out_dev(RqCuda *ctx, int lin_layer, const float *rows_dev, float 
  *
  * A 4-bit weight matrix of n outputs x k inputs, laid out on the device once (RqCudaQ4).  levels: [n][k / 2] bytes, input 2 j
  * in the low half of byte j, input 2 j + 1 in the high half, each the level (-8 .. 7) + 8; scales: [n][k / gs] IEEE half bits;
- * weight = level x scale.  gs: 32, 64 or 128, dividing k.  _new takes host pointers, _new_dev device pointers (both return when the
- * matrix is complete; the sources may then be freed).  Matrices are freed before their context. */
+ * weight = level x scale.  gs: 32, 64 or 128, dividing k.  _new takes host pointers, _new_dev device pointers (levels 4-byte aligned; both
+ * return when the matrix is complete, the sources may then be freed).  Matrices are freed before their context. */
 typedef struct RqCudaQ4 RqCudaQ4;
 int rq_cuda_q4_new(RqCuda *ctx, int n, int k, int gs, const unsigned char *levels, const unsigned short *scales, RqCudaQ4 **w);
 int rq_cuda_q4_new_dev(RqCuda *ctx, int n, int k, int gs, const unsigned char *levels_dev, const unsigned short *scales_dev, RqCudaQ4 **w);
