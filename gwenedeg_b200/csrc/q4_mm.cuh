@@ -85,6 +85,13 @@ cudaError_t launch_q4_pack(const uint8_t *levels, const __half *scales, const Q4
     return cudaGetLastError();
 }
 
+// The rows' scales: written by the kernel before this one, which may still run when this one starts, so they are no constants of this kernel
+// (the read-only path may hold a line from before the write, and the compiler may move such a load over pdl_wait)
+__device__ __forceinline__ float ld_f32(const float *p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint4 ldg_stream(const uint4 *p) {
     uint4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
@@ -529,7 +536,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
 #pragma unroll
             for (int i = 0; i < XE; i++) {
                 const int e = i * 32 * DW + tid;
-                xn[i] = __ldg(a.xs + (size_t)min(row0 + e / PER, a.rows - 1) * G + min(sl * PER + e % PER, G - 1));
+                xn[i] = ld_f32(a.xs + (size_t)min(row0 + e / PER, a.rows - 1) * G + min(sl * PER + e % PER, G - 1));
             }
 #pragma unroll
             for (int i = 0; i < XW; i++) wn[i] = __ldg(reinterpret_cast<const uint2 *>(wsrc[i] + (size_t)sl * Q4_TILE * PER));
