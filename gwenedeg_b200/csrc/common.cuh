@@ -169,10 +169,13 @@ __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t by
 #endif
 
 // ---- programmatic dependent launch: a kernel launched with launch_pdl may be scheduled while the kernel before it in
-// the stream still runs; it must call pdl_wait() before it touches global memory (the wait returns once the earlier
-// kernel has completed and its writes are visible; in a normal launch it returns at once).  pdl_launch_dependents() lets
-// the next such kernel be scheduled as soon as every CTA of this one has started.  What is saved is the launch latency
+// the stream still runs; it must call pdl_wait() before it touches global memory that another kernel of the stream writes (the wait
+// returns once the earlier kernel has completed and its writes are visible; in a normal launch it returns at once).  What is written once,
+// before the call that launches the kernel is made (a weight matrix), may be read ahead of the wait.  pdl_launch_dependents() lets
+// the next such kernel be scheduled as soon as every CTA of this one has called it.  What is saved is the launch latency
 // between the kernels of one layer, a few microseconds each.
+// A kernel that uses TMEM must not end up waiting for one that waits for it: it takes its TMEM after pdl_wait(), or it follows a kernel of this
+// library that uses none and itself waits before it releases (attn_part_tc_kernel behind tcd_q_prep_kernel).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... KArgs, typename... Args>

@@ -8,6 +8,8 @@
 // and the pairs are added in ascending order from 0.
 // So a row's result does not depend on the other rows of the pass.
 #pragma once
+#include <atomic>
+
 #include "attn_decode.cuh"
 #include "tc05.cuh"
 
@@ -398,7 +400,13 @@ __host__ __device__ constexpr int q4t_scales(int gs, int rt) { return 2 * (Q4_SL
 __host__ __device__ constexpr int q4t_sums(int rt) { return rt * Q4T_FS * 4; }  // one pair's sums [RT][132]
 
 // The registers of a warpgroup: the drain gets what the others do not need.  Per SM: 32 rows or 64 a tile, 20 warps of 96 at launch: 8 x 128 + 8 x 88 +
-// 4 x 40 = 1,888 of 1,920; 128 rows, 16 warps of 128: 8 x 184 + 4 x 96 + 4 x 40 = 2,016 of 2,048 (times 32).
+// 4 x 40 = 1,888 of 1,920; 128 rows, 16 warps of 128: 8 x 184 + 4 x 96 + 4 x 40 = 2,016 of 2,048 (times 32).  Two things rest on the numbers at launch
+// (61,440 or 65,536 registers a CTA), which launch_q4_tiles therefore checks: the split has to fit, or the drain waits for registers for ever;
+// and no two of these CTAs fit an SM, so that CTAs of two clusters cannot each wait for the TMEM that the other's holds.
+__host__ __device__ constexpr int q4t_launch_regs(int rt) { return rt == 128 ? 128 : 96; }
+__host__ __device__ constexpr int q4t_drain_regs(int rt) { return rt == 128 ? 184 : 128; }
+__host__ __device__ constexpr int q4t_unpack_regs(int rt) { return rt == 128 ? 96 : 88; }
+constexpr int Q4T_ISSUE_REGS = 40;
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -490,13 +498,15 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
 #pragma unroll
         for (int i = 0; i < 4; i++) fetch(cu + CU * i, i);
     }
-    pdl_launch_dependents();
     if (tid == 0) {
         for (int i = 0; i < 4; i++) mbar_init(full + i, 5), mbar_init(empty + i, 1);
         for (int i = 0; i < 2; i++) mbar_init(dfull + i, 1), mbar_init(dempty + i, DW);
         mbar_init(&done, 1);
         mbar_fence_init();
     }
+    // TMEM is taken after the wait and before the next kernel may start: a CTA that waits for another kernel holds none, and none
+    // that starts beside this CTA can take it first, so that no two kernels wait for each other
+    pdl_wait();
     if (warp == DW + UW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -505,10 +515,10 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tmem_slot;
-    pdl_wait();
+    pdl_launch_dependents();
 
     if (warp < DW) {
-        setmaxnreg_inc<RT == 128 ? 184 : 128>();
+        setmaxnreg_inc<q4t_drain_regs(RT)>();
         // ---- drain: the warp's 32 outputs x RC rows in accumulator-fragment layout, output 8 k + lane / 4, rows col0 + 8 i + 2 (lane % 4) + 0, 1
         const int quad = warp & 3, col0 = (warp >> 2) * RC, g4 = lane >> 2, t2 = 2 * (lane & 3);
         const uint32_t mine = tbase + ((uint32_t)(quad * 32) << 16) + col0;
@@ -645,7 +655,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
             if (sl + 1 < sl1) put_scales(sl + 1, slot ^ 1);
         }
     } else if (u < UW) {
-        setmaxnreg_dec<RT == 128 ? 96 : 88>();
+        setmaxnreg_dec<q4t_unpack_regs(RT)>();
         bool ok = true;
         const int f = lane & 15, h = lane >> 4;
         uint8_t *out[4];  // the lane's four 16-byte places in the first tile of its part
@@ -680,7 +690,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
         if (lane == 0 && *reinterpret_cast<volatile int *>(err) != 0)  // a wait ran out: the copies in flight get a bounded time to land
             for (int i = 0; i < (1 << lst); i++) mbar_drain(full + i, 0), mbar_drain(full + i, 1);
     } else {
-        setmaxnreg_dec<40>();
+        setmaxnreg_dec<Q4T_ISSUE_REGS>();
         if (u == UW && elect_one()) {
             // ---- MMA issue
             constexpr uint32_t idesc = umma_idesc_i8(128, RT, 0, 0, 1, 1);
@@ -812,6 +822,18 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
     auto kern = q4_tiles_kernel<GS, RT, GATED>;
+    static_assert(Q4T_DRAIN * q4t_drain_regs(RT) + q4t_unpack(RT) * q4t_unpack_regs(RT) + 4 * Q4T_ISSUE_REGS <= q4t_threads(RT) / 32 * q4t_launch_regs(RT), "split of the registers");
+    static_assert(2 * q4t_threads(RT) * q4t_launch_regs(RT) > 65536, "one CTA per SM");
+    static std::atomic<bool> checked[64];
+    int dev = -1;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !checked[dev]) {
+        cudaFuncAttributes fa;
+        const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+        if (e != cudaSuccess) return e;
+        if (fa.numRegs != q4t_launch_regs(RT)) return cudaErrorInvalidKernelImage;  // (built by another compiler: see q4t_launch_regs)
+        if (dev >= 0 && dev < 64) checked[dev] = true;
+    }
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -26,6 +26,15 @@ def test_rows_are_not_read_as_constants():
         assert not re.search(r"\ba\.x[qs]\b", call), call
 
 
+def test_tensor_memory_is_taken_after_the_wait_and_before_the_next_kernel():
+    """Otherwise a kernel that holds tensor memory could wait for one that needs it."""
+    code = source("q4_mm.cuh")
+    code = code[code.index("q4_tiles_kernel(const"):code.index("cudaError_t launch_q4_tiles")]
+    at = [code.index(x) for x in ("pdl_wait()", "tcgen05.alloc", "pdl_launch_dependents()", "setmaxnreg_inc")]
+    assert at == sorted(at)
+    assert code.count("pdl_wait()") == code.count("tcgen05.alloc") == code.count("pdl_launch_dependents()") == 1
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 40, 100, 300])
 def test_norm_and_product_in_turn_on_the_same_rows_without_a_wait(ctx, dev, rows):
