@@ -11,14 +11,10 @@
 #include <atomic>
 
 #include "attn_decode.cuh"
+#include "q4_plan.h"
 #include "tc05.cuh"
 
 namespace rq {
-
-constexpr int Q4_TILE = 16;    // outputs per tile of the layout
-constexpr int Q4_CHUNK = 128;  // inputs per chunk: a (tile, chunk) is 1 KB
-constexpr int Q4_SLICE = 512;  // inputs per slice of the sum's order
-constexpr int Q4_PAIR = 1024;  // ... and per pair of slices
 
 // A weight matrix on the device.  levels: [tiles][chunks][16 outputs][4 pieces of 16 bytes]; piece t, 32-bit word s holds the inputs
 // 32 s + 8 t + 0..7 of the chunk: byte b has input b in its low half and input 4 + b in its high half, as 4-bit two's complement.
@@ -392,12 +388,9 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
 // puts on the multiply-add pipe) 5 %, three unpack warps instead of eight at 32 and 64 rows 40 %.
 // With few tiles the inputs are split over the C CTAs of a cluster at multiples of 1,024: every CTA leaves the sums of its pairs of slices
 // in its shared memory and each CTA adds up its share of the rows in the one order, reading from the others'.
-constexpr int Q4T_DRAIN = 8, Q4T_FS = 132, Q4T_BAND = 12;
+constexpr int Q4T_DRAIN = 8, Q4T_BAND = 12;
 __host__ __device__ constexpr int q4t_unpack(int rt) { return rt == 128 ? 4 : 8; }  // unpack warps
 __host__ __device__ constexpr int q4t_threads(int rt) { return 32 * (Q4T_DRAIN + q4t_unpack(rt) + 4); }  // (the MMA warp's warpgroup has three idle warps)
-__host__ __device__ constexpr int q4t_stage(int rt) { return 16384 + rt * 128; }
-__host__ __device__ constexpr int q4t_scales(int gs, int rt) { return 2 * (Q4_SLICE / gs) * (rt + 128) * 4; }  // two slices' scales of the rows and of the outputs
-__host__ __device__ constexpr int q4t_sums(int rt) { return rt * Q4T_FS * 4; }  // one pair's sums [RT][132]
 
 // The registers of a warpgroup: the drain gets what the others do not need.  Per SM: 32 rows or 64 a tile, 20 warps of 96 at launch: 8 x 128 + 8 x 88 +
 // 4 x 40 = 1,888 of 1,920; 128 rows, 16 warps of 128: 8 x 184 + 4 x 96 + 4 x 40 = 2,016 of 2,048 (times 32).  Two things rest on the numbers at launch
@@ -807,14 +800,8 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
 }
 
 template <int GS, int RT, bool GATED>
-cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cudaStream_t stream) {
-    const int pairs = (a.w.slices + 1) / 2, np = (pairs + C - 1) / C;
-    C = (pairs + np - 1) / np;
-    const int P = GATED && a.hq && GS == 128 ? 2 : 1;
-    const int fixed = 1024 + q4t_scales(GS, RT) + q4t_sums(RT) * (C > 1 ? np : 1), most = 226 * 1024;
-    const int lst = (most - fixed) / q4t_stage(RT) >= 4 ? 2 : 1;
-    const int smem = fixed + (q4t_stage(RT) << lst);
-    if (smem > most) return cudaErrorInvalidValue;
+cudaError_t launch_q4_tiles(const Q4Args &a, const Q4Plan &plan, Q4EncodeFn enc, int *err, cudaStream_t stream) {
+    const int C = plan.c, P = plan.p;
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)a.w.k, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.w.k};
     const cuuint32_t box[2] = {Q4_CHUNK, RT}, es[2] = {1, 1};
@@ -834,14 +821,14 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
         if (fa.numRegs != q4t_launch_regs(RT)) return cudaErrorInvalidKernelImage;  // (built by another compiler: see q4t_launch_regs)
         if (dev >= 0 && dev < 64) checked[dev] = true;
     }
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     const int tiles = GATED ? 4 : 8;
     const int fts = (a.w.tiles + tiles - 1) / tiles, rts = (a.rows + RT - 1) / RT;
     cfg.gridDim = dim3((unsigned)(C * fts * rts));
     cfg.blockDim = dim3(q4t_threads(RT));
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = plan.smem;
     cfg.stream = stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -852,31 +839,7 @@ cudaError_t launch_q4_tiles(const Q4Args &a, int C, Q4EncodeFn enc, int *err, cu
     at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = C * P > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, a, map, lst, np, C, P, err);
-}
-
-// Rows per tile and CTAs along the inputs with the least estimated time, in clocks.  CTAs run one per SM, in waves; a CTA costs 6,000 to start
-// and end (2,500 more in a cluster) and a chunk of 128 inputs a part for its stage and a part per group that is drained, as measured:
-// 32 rows 750 + 190, 64 rows 700 + 500, 128 rows 650 + 960.
-struct Q4Plan {
-    int rt, c;
-};
-inline Q4Plan q4_plan(const Q4Args &a, bool gated, int n_sm) {
-    const int pairs = (a.w.slices + 1) / 2, tiles = (a.w.tiles + (gated ? 3 : 7)) / (gated ? 4 : 8), P = gated && a.hq && a.w.gs == 128 ? 2 : 1;
-    Q4Plan best = {128, 1};
-    double least = 1e300;
-    for (int rt = 32; rt <= 128; rt *= 2) {
-        const double chunk = rt == 128 ? 650.0 + 960.0 * (Q4_CHUNK / a.w.gs) : rt == 64 ? 700.0 + 500.0 * (Q4_CHUNK / a.w.gs) : 750.0 + 190.0 * (Q4_CHUNK / a.w.gs);
-        for (int c = 1; c * P <= 8 && c <= pairs; c++) {
-            const int np = (pairs + c - 1) / c;
-            if ((pairs + np - 1) / np != c) continue;
-            if (1024 + q4t_scales(a.w.gs, rt) + q4t_sums(rt) * (c > 1 ? np : 1) + 2 * q4t_stage(rt) > 226 * 1024) continue;
-            const long long ctas = (long long)c * tiles * ((a.rows + rt - 1) / rt), slots = n_sm / (c * P) * (c * P);
-            const double time = (double)((ctas + slots - 1) / slots) * (6000.0 + (c > 1 ? 2500.0 : 0.0) + (double)np * (Q4_PAIR / Q4_CHUNK) * chunk);
-            if (time < least) least = time, best = {rt, c};
-        }
-    }
-    return best;
+    return cudaLaunchKernelEx(&cfg, kern, a, map, plan.lst, plan.np, C, P, err);
 }
 
 // Up to this many rows the kernel for few rows is the faster one, in blocks of 8 or 16 rows (a block of 16 costs 1.75 blocks of 8).  Measured with
@@ -890,10 +853,10 @@ cudaError_t launch_q4_gs(const Q4Args &a, bool gated, int n_sm, Q4EncodeFn enc, 
         if (7 * ((a.rows + 15) / 16) > 4 * ((a.rows + 7) / 8)) return launch_q4_rows<GS, 1, GATED_>(a, stream); \
         return launch_q4_rows<GS, 2, GATED_>(a, stream);                                    \
     }                                                                                       \
-    const Q4Plan plan = q4_plan(a, GATED_, n_sm);                                           \
-    if (plan.rt == 32) return launch_q4_tiles<GS, 32, GATED_>(a, plan.c, enc, err, stream); \
-    if (plan.rt == 64) return launch_q4_tiles<GS, 64, GATED_>(a, plan.c, enc, err, stream); \
-    return launch_q4_tiles<GS, 128, GATED_>(a, plan.c, enc, err, stream)
+    const Q4Plan plan = q4_plan(a.rows, a.w.tiles, a.w.slices, GS, GATED_, a.hq != nullptr, n_sm); \
+    if (plan.rt == 32) return launch_q4_tiles<GS, 32, GATED_>(a, plan, enc, err, stream); \
+    if (plan.rt == 64) return launch_q4_tiles<GS, 64, GATED_>(a, plan, enc, err, stream); \
+    return launch_q4_tiles<GS, 128, GATED_>(a, plan, enc, err, stream)
     if (gated) { Q4_BY_ROWS(true); }
     Q4_BY_ROWS(false);
 #undef Q4_BY_ROWS

@@ -1,7 +1,9 @@
 """The products around the attention, launched one behind the other: what a kernel may do while the kernel before it still runs,
 several host threads at once, and the one order of the sums."""
+import ctypes as C
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -15,6 +17,43 @@ def source(name):
     """A source file without its comments."""
     txt = open(os.path.join(CSRC, name)).read()
     return re.sub(r"//[^\n]*", "", re.sub(r"/\*.*?\*/", "", txt, flags=re.S))
+
+
+# ---- the plan of the products with many rows --------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """The library's own choice of tile and split, built for the host: (rows, n, k, gs, gated, quant) -> rt, c, p, np, lst, smem."""
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text('#include "q4_plan.h"\nextern "C" void plan(int rows, int tiles, int slices, int gs, int gated, int quant, int n_sm, int *o) {\n'
+                                '  const rq::Q4Plan p = rq::q4_plan(rows, tiles, slices, gs, gated, quant, n_sm);\n'
+                                '  const int v[6] = {p.rt, p.c, p.p, p.np, p.lst, p.smem};\n  for (int i = 0; i < 6; i++) o[i] = v[i];\n}\n')
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I", CSRC, str(d / "plan.cpp"), "-o", str(d / "plan.so")])
+    lib = C.CDLL(str(d / "plan.so"))
+
+    def run(rows, n, k, gs, gated=False, quant=False, n_sm=148):
+        o = (C.c_int * 6)()
+        lib.plan(rows, -(-n // 16), -(-k // 512), gs, int(gated), int(quant), n_sm, o)
+        return dict(zip(("rt", "c", "p", "np", "lst", "smem"), o))
+
+    return run
+
+
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("gated,quant", [(False, False), (True, False), (True, True)])
+def test_every_plan_fits_its_shared_memory(plan, gs, gated, quant):
+    """Up to the longest inputs that a matrix may have: the pairs of slices cover the inputs, no CTA of a split is without one, and the
+    shared memory holds what the kernel puts there, counted here in exact integers."""
+    for k in [32, 512, 544, 1024, 1056, 4096, 12288, 25600, 131072] + [1 << b for b in range(18, 31)] + [(1 << 30) - 128, 3 << 27, 130154496, 260309 * 1024]:
+        k = max(gs, k // gs * gs)
+        for n in (128, 4096, 65536, 1 << 21):
+            for rows in (57, 64, 300, 2048, 16384):
+                p = plan(rows, n, k, gs, gated, quant)
+                pairs = -(-(-(-k // 512)) // 2)
+                assert p["rt"] in (32, 64, 128) and 1 <= p["c"] * p["p"] <= 8 and p["lst"] in (1, 2), (k, n, rows, p)
+                assert (p["c"] - 1) * p["np"] < pairs <= p["c"] * p["np"], (k, n, rows, p)
+                need = 1024 + ((16384 + 128 * p["rt"]) << p["lst"]) + 2 * (512 // gs) * (p["rt"] + 128) * 4 + p["rt"] * 132 * 4 * (p["np"] if p["c"] > 1 else 1)
+                assert p["smem"] == need <= 226 * 1024, (k, n, rows, p)
+                assert p["p"] == (2 if gated and quant and gs == 128 else 1)
 
 
 # ---- a kernel beside the kernel before it -----------------------------------------------------------------------------
