@@ -347,8 +347,11 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
     auto kern = a.w.slices > NW ? q4_rows_kernel<GS, NT, GATED, true, 256> : q4_rows_kernel<GS, NT, GATED, false, 256>;
     if constexpr (WIDE)
         if (wide) kern = q4_rows_kernel<GS, NT, GATED, false, 768>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (the most that any shape asks of this kernel, not what this one does: the value belongs to the kernel, and another thread's call may be
+    // between its own setting and its launch)
+    const int most = (WIDE && wide ? 24 : 8) * q4r_warp_bytes(GS, NT);
+    if (most > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
@@ -821,7 +824,8 @@ cudaError_t launch_q4_tiles(const Q4Args &a, const Q4Plan &plan, Q4EncodeFn enc,
         if (fa.numRegs != q4t_launch_regs(RT)) return cudaErrorInvalidKernelImage;  // (built by another compiler: see q4t_launch_regs)
         if (dev >= 0 && dev < 64) checked[dev] = true;
     }
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
+    // (the same value in every call: it belongs to the kernel, and another thread's call may be between its own setting and its launch)
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4T_SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     const int tiles = GATED ? 4 : 8;

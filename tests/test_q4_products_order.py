@@ -4,11 +4,12 @@ import ctypes as C
 import os
 import re
 import subprocess
+import threading
 
 import numpy as np
 import pytest
 
-from tests.test_q4_products import ctx, dev, matrix, packed  # noqa: F401  (ctx, dev: fixtures)
+from tests.test_q4_products import Dev, ctx, dev, matrix, packed, rows8  # noqa: F401  (ctx, dev: fixtures)
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gwenedeg_b200", "csrc")
 
@@ -99,3 +100,48 @@ def test_norm_and_product_in_turn_on_the_same_rows_without_a_wait(ctx, dev, rows
             ctx.mm_q4_dev(w, rows, q, s, outs[i])
     for i in range(turns):
         assert np.array_equal(dev.get(outs[i], (rows, n)).view(np.uint32), alone[i].view(np.uint32)), i
+
+
+# ---- several host threads ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,ks", [(64, (20480, 512, 12288)), (1, (12288, 6656, 5120)), (200, (12288, 4096, 1024))])
+@pytest.mark.parametrize("gated", [False, True])
+def test_contexts_in_threads_of_their_own(rows, ks, gated):
+    """One context per host thread, all on one device, with the same kernels at shapes that want different amounts of shared memory:
+    no call is refused and the results are those of the calls made alone."""
+    import gwenedeg_b200 as gw
+    rng = np.random.default_rng(rows)
+    n, gs, turns = 256, 64, 400
+    jobs = []
+    for k in ks:
+        c = gw.Context(0, n_attn=1, n_heads=8, n_kv_heads=2, head_dim=128, max_rows=256)
+        d = Dev(c)
+        m = [c.q4_new(packed(lev), sc, gs) for lev, sc in (matrix(rng, n, k, gs), matrix(rng, n, k, gs))]
+        xq, xs = rows8(rng, rows, k, gs)
+        q, s, o = d.put(xq), d.put(xs * np.float32(0.1)), d.room((rows, n), np.float32)
+        call = (lambda c=c, m=m, q=q, s=s, o=o: c.ffn_q4_dev(m[0], m[1], rows, q, s, o, None, None)) if gated else (lambda c=c, m=m, q=q, s=s, o=o: c.mm_q4_dev(m[0], rows, q, s, o))
+        call()
+        jobs.append((c, d, call, o, d.get(o, (rows, n))))
+    failed, start = [], threading.Barrier(len(jobs))
+
+    def work(c, call):
+        start.wait()
+        try:
+            for _ in range(turns):
+                call()
+            c.sync()
+        except Exception as e:
+            failed.append(e)
+
+    ts = [threading.Thread(target=work, args=(c, call)) for c, _, call, _, _ in jobs]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    got = [d.get(o, (rows, n)) for _, d, _, o, _ in jobs]
+    for c, d, *_ in jobs:
+        d.free()
+        c.close()
+    assert not failed, failed
+    for g, (*_, alone) in zip(got, jobs):
+        assert np.array_equal(g.view(np.uint32), alone.view(np.uint32))
