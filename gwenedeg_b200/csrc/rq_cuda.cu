@@ -176,15 +176,13 @@ typedef CUresult (*TmEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, v
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static TmEncodeFn tm_encode() {
     // the driver's tensor-map encoder, looked up through the runtime (no link-time dependency on libcuda)
-    static TmEncodeFn fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
+    // (initialised once, under the language's own lock: contexts in several host threads may ask at the same time)
+    static const TmEncodeFn fn = [] {
         cudaDriverEntryPointQueryResult qr;
         void *p = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess)
-            fn = (TmEncodeFn)p;
-    }
+        const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess;
+        return found ? (TmEncodeFn)p : nullptr;
+    }();
     return fn;
 }
 

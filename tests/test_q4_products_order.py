@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import re
 import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -145,3 +146,41 @@ def test_contexts_in_threads_of_their_own(rows, ks, gated):
     assert not failed, failed
     for g, (*_, alone) in zip(got, jobs):
         assert np.array_equal(g.view(np.uint32), alone.view(np.uint32))
+
+
+FIRST_CALLS = """
+import sys, threading
+import numpy as np
+sys.path.insert(0, sys.argv[1])
+import gwenedeg_b200 as gw
+rows, n, k, gs, jobs, failed = 64, 128, 512, 64, [], []
+for _ in range(8):
+    c = gw.Context(0, n_attn=1, n_heads=8, n_kv_heads=2, head_dim=128, max_rows=64)
+    m = c.q4_new(np.full((n, k // 2), 0x99, np.uint8), np.ones((n, k // gs), np.float16), gs)
+    jobs.append((c, m, c.to_device(np.ones((rows, k), np.int8)), c.to_device(np.ones((rows, k // gs), np.float32)), c.to_device(np.zeros((rows, n), np.float32))))
+start = threading.Barrier(len(jobs))
+def work(c, m, q, s, o):
+    start.wait()
+    try:
+        c.mm_q4_dev(m, rows, q, s, o)
+        c.sync()
+    except Exception as e:
+        failed.append(e)
+ts = [threading.Thread(target=work, args=j) for j in jobs]
+[t.start() for t in ts]
+[t.join() for t in ts]
+assert not failed, failed
+for c, m, q, s, o in jobs:
+    got = np.empty((rows, n), np.float32)
+    c.d2h(got, o)
+    c.sync()
+    assert (got == k).all()
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_calls_of_a_process_in_several_threads():
+    """What the library looks up once per process is there for every thread that asks, the first ones at the same time included."""
+    for _ in range(2):
+        r = subprocess.run([sys.executable, "-c", FIRST_CALLS, os.path.dirname(os.path.dirname(CSRC))], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stderr[-600:]
