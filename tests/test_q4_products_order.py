@@ -10,7 +10,7 @@ import threading
 import numpy as np
 import pytest
 
-from tests.test_q4_products import Dev, ctx, dev, matrix, packed, rows8  # noqa: F401  (ctx, dev: fixtures)
+from tests.test_q4_products import SLICE, Dev, ctx, dev, matrix, packed, product, quantised, rows8  # noqa: F401  (ctx, dev: fixtures)
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gwenedeg_b200", "csrc")
 
@@ -19,6 +19,119 @@ def source(name):
     """A source file without its comments."""
     txt = open(os.path.join(CSRC, name)).read()
     return re.sub(r"//[^\n]*", "", re.sub(r"/\*.*?\*/", "", txt, flags=re.S))
+
+
+# ---- the one order of the sums ----------------------------------------------------------------------------------------
+def fma32(a, b, c):
+    """a b + c of fp32 arrays with one rounding.  The product is exact in 64 bits; the sum is rounded to odd there (by its exact
+    remainder), which keeps enough for the rounding to 24 bits to be the only one that counts (Boldo and Melquiond 2008)."""
+    p, c = a.astype(np.float64) * b.astype(np.float64), c.astype(np.float64)
+    s = p + c
+    t = s - p
+    rest = (p - (s - t)) + (c - t)  # p + c - s, exactly
+    bits = s.view(np.int64)
+    even = (rest != 0) & (bits & 1 == 0)
+    away = (rest > 0) == (s > 0)  # the exact sum is further from zero than s
+    return np.where(even, np.where(away, bits + 1, bits - 1), bits).view(np.float64).astype(np.float32)
+
+
+def in_order(xq, xs, lev, sc, gs):
+    """The product in fp32 in the order that rq_cuda.h states, operation for operation."""
+    r, k = xq.shape
+    n, G = lev.shape[0], k // gs
+    D = np.einsum("rgi,ngi->rng", xq.reshape(r, G, gs).astype(np.float64), lev.reshape(n, G, gs).astype(np.float64), optimize=True)
+    slices = []
+    for s in range(0, G, SLICE // gs):
+        p = np.zeros((r, n), np.float32)
+        for g in range(s, min(G, s + SLICE // gs)):
+            t = (D[:, :, g] * sc[None, :, g].astype(np.float64)).astype(np.float32)  # (exact in 64 bits, rounded once)
+            p = fma32(t, np.broadcast_to(xs[:, None, g], t.shape), p)
+        slices.append(p)
+    y = np.zeros((r, n), np.float32)
+    for s in range(0, len(slices), 2):
+        y = y + (slices[s] + slices[s + 1] if s + 1 < len(slices) else slices[s])
+    return y
+
+
+def test_the_fused_operation_of_these_tests_is_rounded_once():
+    from fractions import Fraction
+    rng = np.random.default_rng(0)
+    a, b, c = ((rng.standard_normal(4000) * 2.0 ** rng.integers(-14, 14, 4000)).astype(np.float32) for _ in range(3))
+    c[:1000] = -(a[:1000].astype(np.float64) * b[:1000]).astype(np.float32)  # cancelled down to the product's own rounding error
+    a[1000:2000] = np.float32(1) + a[1000:2000] * np.float32(2.0 ** -30)  # borders: sums half way between two fp32 numbers, and next to them
+    c[1000:2000] = np.ldexp(b[1000:2000], 24) * rng.choice([1, -1, 3], 1000).astype(np.float32)
+    got = fma32(a, b, c)
+    for x, y, z, g in zip(a, b, c, got):
+        want = Fraction(float(x)) * Fraction(float(y)) + Fraction(float(z))
+        near = abs(Fraction(float(g)) - want)
+        lo, hi = np.nextafter(g, np.float32(-np.inf)), np.nextafter(g, np.float32(np.inf))
+        others = [abs(Fraction(float(o)) - want) for o in (lo, hi)]
+        assert near < min(others) or (near == min(others) and int(g.view(np.int32)) % 2 == 0)
+
+
+@pytest.mark.parametrize("k,gs", [(2080, 32), (4160, 64), (2176, 128)])
+def test_the_stated_order_is_within_the_bound(k, gs):
+    rng = np.random.default_rng(k)
+    lev, sc = matrix(rng, 24, k, gs)
+    xq, xs = rows8(rng, 10, k, gs)
+    want, tol = product(xq, xs, lev, sc, gs)
+    assert (np.abs(in_order(xq, xs, lev, sc, gs) - want) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k,gs", [(96, 32), (544, 32), (2080, 32), (5664, 32), (192, 64), (4160, 64), (13376, 64), (128, 128), (2176, 128), (13440, 128)])
+def test_products_have_the_bits_of_the_stated_order(ctx, dev, k, gs):
+    """An odd and an even number of slices, a last chunk that is not full, few rows and many, split over a cluster or not."""
+    rng = np.random.default_rng(k + gs)
+    n, most = 145, 150
+    lev, sc = matrix(rng, n, k, gs)
+    xq, xs = rows8(rng, most, k, gs)
+    want = in_order(xq, xs, lev, sc, gs)
+    w = ctx.q4_new(packed(lev), sc, gs)
+    q, s, out = dev.put(xq), dev.put(xs), dev.room((most, n), np.float32)
+    for rows in (1, 8, 9, 25, 40, 57, 64, 100, most):
+        ctx.mm_q4_dev(w, rows, q, s, out)
+        assert np.array_equal(dev.get(out, (rows, n)).view(np.uint32), want[:rows].view(np.uint32)), rows
+
+
+# ---- the order of the tiles -------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,gs", [(300, 3400, 512, 64), (200, 1552, 1056, 32), (512, 2000, 640, 128), (70, 4700, 2176, 128), (57, 40, 32, 32), (64, 17, 64, 64),
+                                         (100, 130, 96, 32), (200, 16, 128, 128)])
+def test_products_over_several_bands_of_tiles(ctx, dev, rows, n, k, gs):
+    """More outputs than one band of tiles has, with a last band and a last tile that are not full; inputs shorter than a chunk."""
+    rng = np.random.default_rng(rows + n)
+    lev, sc = matrix(rng, n, k, gs)
+    xq, xs = rows8(rng, rows, k, gs)
+    w = ctx.q4_new(packed(lev), sc, gs)
+    out = dev.room(rows * n + 64, np.float32, fill=-7.5)
+    ctx.mm_q4_dev(w, rows, dev.put(xq), dev.put(xs), out)
+    got = dev.get(out, rows * n + 64)
+    assert (got[rows * n:] == -7.5).all()
+    assert np.array_equal(got[:rows * n].reshape(rows, n).view(np.uint32), in_order(xq, xs, lev, sc, gs).view(np.uint32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,gs", [(300, 1728, 512, 64), (200, 1664, 1152, 128), (260, 2432, 256, 128), (130, 1600, 544, 32), (60, 128, 128, 128), (57, 32, 32, 32)])
+def test_gated_products_over_several_bands_of_tiles(ctx, dev, rows, n, k, gs):
+    """The same for the gated product with its rows in 8 bits; groups of 128 outputs lie across two tiles of a pair."""
+    rng = np.random.default_rng(rows + n)
+    ms = [matrix(rng, n, k, gs) for _ in range(2)]
+    xq, xs = rows8(rng, rows, k, gs)
+    xs *= np.float32(0.3)
+    gate, up = (ctx.q4_new(packed(lev), sc, gs) for lev, sc in ms)
+    q, s = dev.put(xq), dev.put(xs)
+    h, hq, hs = dev.room((rows, n), np.float32), dev.room(rows * n + 64, np.int8, fill=99), dev.room(rows * (n // gs) + 64, np.float32, fill=-7.5)
+    ctx.ffn_q4_dev(gate, up, rows, q, s, h, hq, hs)
+    got, lev, sc = dev.get(h, (rows, n)), dev.get(hq, rows * n + 64, np.int8), dev.get(hs, rows * (n // gs) + 64)
+    assert (lev[rows * n:] == 99).all() and (sc[rows * (n // gs):] == -7.5).all()
+    g, u = (in_order(xq, xs, *m, gs).astype(np.float64) for m in ms)
+    want = g / (1.0 + np.exp(-g)) * u
+    # on exactly these g and u: e^-g (2 units in the last place = 4 half steps), 1 + e^-g, the division, the product: 7 half steps
+    assert (np.abs(got - want) <= 8 * 2.0 ** -24 * np.abs(want) + 1e-37).all()
+    wl, top = quantised(got, gs)
+    assert np.array_equal(lev[:rows * n].reshape(rows, n), wl)
+    assert np.array_equal(sc[:rows * (n // gs)].reshape(rows, -1), top * np.float32(1.0 / 127.0))
 
 
 # ---- the plan of the products with many rows --------------------------------------------------------------------------
