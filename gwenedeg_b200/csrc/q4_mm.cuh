@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
     auto totals = [&](int r, int f, float *t) {
         if (C == 1) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[i] = sums[r * Q4T_FS + f + 32 * i] * 0.0625f;
+            for (int i = 0; i < 4; i++) t[i] = (0.0f + sums[r * Q4T_FS + f + 32 * i]) * 0.0625f;  // (from 0: a vanished -0 is 0)
             return;
         }
         t[0] = t[1] = t[2] = t[3] = 0.0f;

@@ -94,6 +94,30 @@ def test_products_have_the_bits_of_the_stated_order(ctx, dev, k, gs):
         assert np.array_equal(dev.get(out, (rows, n)).view(np.uint32), want[:rows].view(np.uint32)), rows
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("k,gs", [(64, 32), (512, 64), (1024, 128), (4096, 128)])
+def test_the_sign_of_a_zero_does_not_depend_on_the_other_rows(ctx, dev, k, gs, gated):
+    """Scales so small that the products vanish: the sums are zeros, and the same ones in both kernels."""
+    n, most = 64, 200
+    rng = np.random.default_rng(k)
+    lev = rng.integers(-8, 8, (n, k)).astype(np.int8)
+    lev[:32] = -1
+    w = ctx.q4_new(packed(lev), np.full((n, k // gs), 2.0 ** -20, np.float16), gs)
+    xq = np.ones((most, k), np.int8)
+    xs = np.full((most, k // gs), 2.0 ** -149, np.float32)
+    q, s, out = dev.put(xq), dev.put(xs), dev.room((most, n), np.float32)
+    got = []
+    for rows in (1, 40, 64, most):
+        if gated:
+            ctx.ffn_q4_dev(w, w, rows, q, s, out, None, None)
+        else:
+            ctx.mm_q4_dev(w, rows, q, s, out)
+        got.append(dev.get(out, (rows, n)))
+        assert (got[-1] == 0).all()
+        assert (got[-1].view(np.uint32) == got[0].view(np.uint32)).all(), rows
+
+
 # ---- the order of the tiles -------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,n,k,gs", [(300, 3400, 512, 64), (200, 1552, 1056, 32), (512, 2000, 640, 128), (70, 4700, 2176, 128), (57, 40, 32, 32), (64, 17, 64, 64),
