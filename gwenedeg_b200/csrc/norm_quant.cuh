@@ -79,10 +79,11 @@ __global__ void __launch_bounds__(1024) add_norm_quant_kernel(const NormQuantArg
 #pragma unroll
             for (int o = GS / 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             if (i < n4) {
+                const float t = quant_top(m);
                 char4 q;
-                q.x = wo_quant_level(u.x, m), q.y = wo_quant_level(u.y, m), q.z = wo_quant_level(u.z, m), q.w = wo_quant_level(u.w, m);
+                q.x = wo_quant_level(u.x, t), q.y = wo_quant_level(u.y, t), q.z = wo_quant_level(u.z, t), q.w = wo_quant_level(u.w, t);
                 reinterpret_cast<char4 *>(a.xq + row * a.dim)[i] = q;
-                if (i % (GS / 4) == 0) a.xs[row * (a.dim / GS) + i / (GS / 4)] = m * (1.0f / 127.0f) * inv;
+                if (i % (GS / 4) == 0) a.xs[row * (a.dim / GS) + i / (GS / 4)] = quant_scale(m) * inv;
             }
         }
         if (a.y && i < n4) reinterpret_cast<float4 *>(a.y + row * a.dim)[i] = make_float4(u.x * inv, u.y * inv, u.z * inv, u.w * inv);

@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(MOST, MOST > 256 ? 1 : NT == 1 && GS >= 64 ? 3
                 }
                 if (r < rows) {
                     const size_t f = (size_t)blockIdx.x * 16 + fo;
-                    a.hq[(size_t)(row0 + r) * W.n + f] = wo_quant_level(h[e], m);
-                    if (f % GS == 0) a.hs[(size_t)(row0 + r) * (W.n / GS) + f / GS] = m * (1.0f / 127.0f);
+                    a.hq[(size_t)(row0 + r) * W.n + f] = wo_quant_level(h[e], quant_top(m));
+                    if (f % GS == 0) a.hs[(size_t)(row0 + r) * (W.n / GS) + f / GS] = quant_scale(m);
                 }
             }
             // (no CTA leaves while another may still read its maxima)
@@ -791,8 +791,8 @@ __global__ void __launch_bounds__(q4t_threads(RT), 1)
                     if (f < W.n) {
                         if (a.out) a.out[at] = v[i];
                         if (a.hq) {
-                            a.hq[at] = wo_quant_level(v[i], __uint_as_float(m[i]));
-                            if (f % GS == 0) a.hs[at / GS] = __uint_as_float(m[i]) * (1.0f / 127.0f);
+                            a.hq[at] = wo_quant_level(v[i], quant_top(__uint_as_float(m[i])));
+                            if (f % GS == 0) a.hs[at / GS] = quant_scale(__uint_as_float(m[i]));
                         }
                     }
                 }

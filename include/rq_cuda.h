@@ -329,7 +329,8 @@ size_t rq_cuda_q4_bytes(const RqCudaQ4 *w); /* device memory it holds */
 /* x' = x + delta per element (delta NULL: x' = x), written to x_out (may be x itself; NULL: not written); then per row
  * inv = 1 / sqrt(mean(x'^2) + eps) and v = w x'; y = v inv (NULL: not written); xq, xs (both NULL: not written): per group of gs
  * values the levels of the library's quantiser (rq_cuda_set_wo_quant) on v and scale = max|v| (1 / 127) inv.  inv cancels out
- * of the levels: they are a function of x', w and the group alone.  dim: a multiple of gs, at most 32768; gs 32, 64 or 128.
+ * of the levels: they are a function of x', w and the group alone.  A group's max|v| counts as at least 2^-119 (smaller ones have no
+ * inverse in fp32), unless all of it is zero: then levels and scale are 0.  dim: a multiple of gs, at most 32768; gs 32, 64 or 128.
  * x, x_out, delta, w, y 16-byte aligned; xq, xs 4-byte aligned. */
 int rq_cuda_add_norm_quant_dev(RqCuda *ctx, int rows, int dim, int gs, const float *x_dev, const float *delta_dev, const float *w_dev,
                                float eps, float *x_out_dev, float *y_dev, signed char *xq_dev, float *xs_dev);
@@ -340,7 +341,7 @@ int rq_cuda_add_norm_quant_dev(RqCuda *ctx, int rows, int dim, int gs, const flo
 int rq_cuda_mm_q4_dev(RqCuda *ctx, const RqCudaQ4 *w, int rows, const signed char *xq_dev, const float *xs_dev, float *out_dev);
 /* The gated feed-forward product in one kernel: h = silu(x gate^T) (x up^T), silu(g) = g / (1 + e^-g), both products as
  * rq_cuda_mm_q4_dev.  h_dev: fp32 [rows][n]; hq_dev, hs_dev: the same rows through the library's quantiser, levels [rows][n] and
- * scales [rows][n / gs] with the matrices' gs (n a multiple of gs then), ready for the down product.  Either h_dev or the pair
+ * scales [rows][n / gs] with the matrices' gs (n a multiple of gs then; small groups as above), ready for the down product.  Either h_dev or the pair
  * may be NULL.  gate and up have the same shape and gs; both may be the same matrix. */
 int rq_cuda_ffn_q4_dev(RqCuda *ctx, const RqCudaQ4 *gate, const RqCudaQ4 *up, int rows, const signed char *xq_dev, const float *xs_dev,
                        float *h_dev, signed char *hq_dev, float *hs_dev);

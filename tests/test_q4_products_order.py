@@ -321,3 +321,55 @@ def test_the_first_calls_of_a_process_in_several_threads():
     for _ in range(2):
         r = subprocess.run([sys.executable, "-c", FIRST_CALLS, os.path.dirname(os.path.dirname(CSRC))], capture_output=True, text=True, timeout=120)
         assert r.returncode == 0, r.stderr[-600:]
+
+
+# ---- groups of very small values --------------------------------------------------------------------------------------
+SMALL = [2.0 ** e for e in (-100, -118, -119, -120, -121, -122, -124, -126, -130, -140)]
+LEAST = 2.0 ** -119  # what a group's largest magnitude counts as at least (rq_cuda.h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64, 128])
+def test_norm_quantises_groups_of_very_small_values(ctx, dev, gs):
+    """Groups whose 127 / max is beyond fp32, down to subnormal numbers: levels and scales stand for the values to half a unit of the
+    least maximum all the same."""
+    rng = np.random.default_rng(gs)
+    eps, rows, dim = 1e-6, len(SMALL), 4 * gs
+    x = rng.uniform(-1, 1, (rows, dim)).astype(np.float64) * np.array(SMALL)[:, None]
+    x[:, ::gs] = np.array(SMALL)[:, None] * np.array([1, -1, 1, -1])  # the largest of each group
+    x[:, 3 * gs:] = 0.0
+    x = x.astype(np.float32)
+    q, s = dev.room((rows, dim), np.int8), dev.room((rows, 4), np.float32)
+    ctx.add_norm_quant_dev(rows, dim, gs, dev.put(x), None, dev.put(np.ones(dim, np.float32)), eps, None, None, q, s)
+    lev, sc = dev.get(q, (rows, dim), np.int8).reshape(rows, 4, gs), dev.get(s, (rows, 4))
+    v = x.astype(np.float64).reshape(rows, 4, gs)
+    top = np.maximum(np.abs(v).max(2), LEAST)
+    inv = 1.0 / np.sqrt((v ** 2).mean((1, 2)) + eps)
+    # half a unit, the quantiser's 0.49999997 for 0.5, and half steps of 127 / max and of the product with a value of at most 127
+    assert (np.abs(lev[:, :3] - 127.0 * v[:, :3] / top[:, :3, None]) <= 0.5 + 4 * 127 * 2.0 ** -24).all()
+    assert (lev[:, 3] == 0).all() and (sc[:, 3] == 0).all()
+    # 1 / 127, the root, the division and three products, each half a step (no sum of squares: eps is all there is)
+    want = (top / 127.0 * inv[:, None])[:, :3]
+    assert (np.abs(sc[:, :3] - want) <= 8 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 20, 100])
+@pytest.mark.parametrize("gs", [32, 64, 128])
+def test_gated_rows_quantise_groups_of_very_small_values(ctx, dev, rows, gs):
+    rng = np.random.default_rng(gs + rows)
+    n, k = len(SMALL) * 128, 128
+    gate, up = (ctx.q4_new(packed(lev), sc, gs) for lev, sc in (matrix(rng, n, k, gs), matrix(rng, n, k, gs)))
+    xq, xs = rows8(rng, rows, k, gs)
+    # h is about g u / 2 for small g: the rows' scales put it where the quantiser's inverse overflows
+    for r in range(rows):
+        xs[r] *= np.float32(np.sqrt(SMALL[r % len(SMALL)]))
+    h, hq, hs = dev.room((rows, n), np.float32), dev.room((rows, n), np.int8), dev.room((rows, n // gs), np.float32)
+    ctx.ffn_q4_dev(gate, up, rows, dev.put(xq), dev.put(xs), h, hq, hs)
+    v = dev.get(h, (rows, n)).astype(np.float64).reshape(rows, -1, gs)
+    lev, sc = dev.get(hq, (rows, n), np.int8).reshape(rows, -1, gs), dev.get(hs, (rows, n // gs))
+    top = np.abs(v).max(2)
+    least = np.maximum(top, LEAST)
+    assert (np.abs(lev - 127.0 * v / least[:, :, None]) <= 0.5 + 4 * 127 * 2.0 ** -24).all()
+    want = np.where(top > 0, least / 127.0, 0.0)  # (the smallest rows may vanish)
+    assert (np.abs(sc - want) <= 2 * 2.0 ** -24 * want).all()
