@@ -178,6 +178,12 @@ __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t by
 // library that uses none and itself waits before it releases (attn_part_tc_kernel behind tcd_q_prep_kernel).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// A kernel that calls pdl_launch_dependents() ahead of its own pdl_wait() (the norm, the products with few rows) lets the next one start while
+// the kernel in front of both still runs.  Its outputs are then no constants of the next kernel, which must not read them through the read-only
+// path (__ldg, taken by the compiler itself for const __restrict__ parameters).  The norm and the products use ordinary loads; the attention and
+// DeltaNet kernels do not (it cost them 1 to 2 %): the host lets the first of them behind such a kernel wait for it in full, by setting
+// this ahead of the launch.
+inline thread_local bool launch_in_order = false;
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
@@ -189,7 +195,8 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = launch_in_order ? 0 : 1;
+    launch_in_order = false;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 

@@ -78,6 +78,7 @@ struct RqCuda {
     double pt_first, pt_more;
     char err[256];
     unsigned long long launches;
+    bool early;  // the last kernel launched lets the next one start ahead of its own wait (launch_in_order)
     // the open pass
     int pass_open, nrows, nseg, total_blocks, pass_kvt, max_np;
     unsigned long long pass_no;  // counts pass_begin calls (RqCudaSeq::stamp)
@@ -171,6 +172,12 @@ static int fail(RqCuda *c, int code, const char *fmt, ...) {
             return fail(c, e_ == cudaErrorMemoryAllocation ? RQ_CUDA_ERR_NOMEM : RQ_CUDA_ERR_DEVICE, "%s: %s", #call, \
                         cudaGetErrorString(e_));                                                             \
     } while (0)
+
+// ahead of the first launch of an attention or DeltaNet call
+static void behind_early(RqCuda *c) {
+    launch_in_order = c->early;
+    c->early = false;
+}
 
 typedef CUresult (*TmEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -948,6 +955,7 @@ int rq_cuda_kv_store_dev(RqCuda *c, int layer, const float *k, const float *v) {
         default: kv_store_kernel<256><<<grid, 256, 0, c->stream>>>(c->d_rows, layer, c->n_kv, c->pass_kvt, k, v, c->d_err); break;
     }
     c->launches++;
+    c->early = false;  // (an ordinary launch: it waits for everything in front of it)
     CU(c, cudaGetLastError());
     return RQ_CUDA_OK;
 }
@@ -990,6 +998,7 @@ int rq_cuda_qk_norm_rope_store_dev(RqCuda *c, int layer, float *q, const float *
     }
 #undef PRODUCER
     c->launches++;
+    c->early = false;
     CU(c, cudaGetLastError());
     return RQ_CUDA_OK;
 }
@@ -1021,6 +1030,7 @@ static int launch_decode_with(RqCuda *c, int layer, const float *q, float *out, 
     a.part = part;
     a.err = c->d_err;
     cudaError_t e;
+    behind_early(c);
     const bool prof = c->prof_on && (size_t)(2 * c->prof_n + 2) <= c->prof_ev.size();
     if (prof) cudaEventRecord(c->prof_ev[2 * c->prof_n], c->stream);
     if (kv_quant(c->pass_kvt) && hd == 128 && !c->exact && may_allocate && c->tc_ready == 0) {
@@ -1401,6 +1411,7 @@ static int launch_prefill(RqCuda *c, int layer, const float *q, float *out) {
     a.split_len = c->pf_split;
     a.part = c->d_part;
     a.err = c->d_err;
+    behind_early(c);
     if (c->pf_quant) {
         // the layer's tiles as f16 (layer 0 of the scratch's views), the query rows rotated; the merge below un-rotates
         // (the same launch rotates the query rows, in z slices of its grid past the segments': a warp per (row, head))
@@ -1691,6 +1702,7 @@ int rq_cuda_dn_chunk_dev(RqCuda *c, int lin_layer, const float *rows, float *out
     a.lw = 2 * m.dn_nk * m.dn_dk + 2 * m.dn_nv * m.dn_dv + 2 * m.dn_nv;
     a.out = out;
     a.err = c->d_err;
+    behind_early(c);
     cudaError_t e = launch_dn_chunk(a, c->stream);
     if (e != cudaSuccess) return fail(c, RQ_CUDA_ERR_DEVICE, "dn_chunk launch: %s", cudaGetErrorString(e));
     c->launches += 2;
@@ -1906,6 +1918,7 @@ int rq_cuda_add_norm_quant_dev(RqCuda *c, int rows, int dim, int gs, const float
     CU(c, cudaSetDevice(c->device));
     const NormQuantArgs a = {x, delta, w, x_out, y, (int8_t *)xq, xs, dim, eps};
     CU(c, launch_add_norm_quant(a, rows, gs, c->stream));
+    c->early = true;
     c->launches++;
     return RQ_CUDA_OK;
 }
@@ -1927,6 +1940,7 @@ int rq_cuda_mm_q4_dev(RqCuda *c, const RqCudaQ4 *w, int rows, const signed char 
     CU(c, cudaSetDevice(c->device));
     const Q4Args a = {w->v, w->v, (const int8_t *)xq, xs, rows, out, nullptr, nullptr};
     CU(c, launch_q4(a, false, c->n_sm, tm_encode(), c->d_err, c->stream));
+    c->early = true;
     c->launches++;
     return RQ_CUDA_OK;
 }
@@ -1945,6 +1959,7 @@ int rq_cuda_ffn_q4_dev(RqCuda *c, const RqCudaQ4 *gate, const RqCudaQ4 *up, int 
     CU(c, cudaSetDevice(c->device));
     const Q4Args a = {g, u, (const int8_t *)xq, xs, rows, h, (int8_t *)hq, hs};
     CU(c, launch_q4(a, true, c->n_sm, tm_encode(), c->d_err, c->stream));
+    c->early = true;
     c->launches++;
     return RQ_CUDA_OK;
 }

@@ -240,6 +240,58 @@ def test_norm_and_product_in_turn_on_the_same_rows_without_a_wait(ctx, dev, rows
         assert np.array_equal(dev.get(outs[i], (rows, n)).view(np.uint32), alone[i].view(np.uint32)), i
 
 
+def test_attention_behind_a_product_waits_for_it_in_full():
+    """The attention and DeltaNet kernels read rows through the read-only path, so their first launch behind a kernel that lets the next
+    one start ahead of its own wait is an ordinary one."""
+    code = source("rq_cuda.cu")
+    for launch in ("= launch_attn_part_tc(t,", "= launch_attn_part<KV_F16>(", "launch_pdl(kv_dequant_f16_kernel<", "= launch_dn_chunk(a,"):
+        body = code[:code.index(launch)]
+        body = body[body.rindex("\n}\n"):]  # the function's part in front of the launch
+        assert "behind_early(c);" in body, launch
+    for entry in ("rq_cuda_add_norm_quant_dev", "rq_cuda_mm_q4_dev", "rq_cuda_ffn_q4_dev"):
+        body = code[code.index("int " + entry):]
+        assert "c->early = true;" in body[:body.index("\n}\n")], entry
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,prefill", [("f16", False), ("q8", False), ("q4", False), ("f16", True), ("q8", True)])
+def test_attention_right_behind_the_product_that_makes_its_queries(kv, prefill):
+    """Query rows written and read again and again with other values, no cache store and no wait in between: the bits of calls that are
+    waited for."""
+    import gwenedeg_b200 as gw
+    rng = np.random.default_rng(31)
+    H, hd, k, gs, ctx_len, turns = 8, 128, 256, 64, 600, 8
+    rows = 64 if prefill else 5
+    c = gw.Context(0, n_attn=1, n_heads=H, n_kv_heads=2, head_dim=hd, max_rows=64)
+    d = Dev(c)
+    lev, sc = matrix(rng, H * hd, k, gs)
+    w = c.q4_new(packed(lev), sc, gs)
+    kvt = dict(f16=gw.KV_F16, q8=gw.KV_Q8, q4=gw.KV_Q4)[kv]
+    seqs = [c.new_seq(ctx_len + 64, kvt) for _ in range(1 if prefill else rows)]
+    for i, s in enumerate(seqs):
+        s.fill_synthetic(ctx_len + (64 if prefill else 1), 3 + i)
+    ins = [tuple(d.put(a) for a in rows8(rng, rows, k, gs)) for _ in range(turns)]
+    q, outs = d.room((rows, H * hd), np.float32), [d.room((rows, H * hd), np.float32) for _ in range(turns)]
+    c.pass_begin([(s, ctx_len, 64 if prefill else 1) for s in seqs])
+    attend = c.attn_prefill_dev if prefill else c.attn_decode_dev
+    alone = []
+    for (xq, xs), o in zip(ins, outs):
+        c.mm_q4_dev(w, rows, xq, xs, q)
+        c.sync()
+        attend(0, q, o)
+        alone.append(d.get(o, (rows, H * hd)))
+    assert not np.array_equal(alone[0], alone[1])
+    for _ in range(10):
+        for (xq, xs), o in zip(ins, outs):
+            c.mm_q4_dev(w, rows, xq, xs, q)
+            attend(0, q, o)
+    for o, a in zip(outs, alone):
+        assert np.array_equal(d.get(o, (rows, H * hd)).view(np.uint32), a.view(np.uint32))
+    c.pass_end(commit=False)
+    d.free()
+    c.close()
+
+
 # ---- several host threads ---------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,ks", [(64, (20480, 512, 12288)), (1, (12288, 6656, 5120)), (200, (12288, 4096, 1024))])
