@@ -158,6 +158,34 @@ def test_gated_products_over_several_bands_of_tiles(ctx, dev, rows, n, k, gs):
     assert np.array_equal(sc[:rows * (n // gs)].reshape(rows, -1), top * np.float32(1.0 / 127.0))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,gs", [(1, 1 << 21, 4224, 64), (70, 1 << 21, 4224, 128), (16384, 70000, 32, 32)])
+def test_products_beyond_32_bit_offsets(rows, n, k, gs):
+    """More than 2^32 bytes of weights, or of outputs: rows and outputs from the front, the middle and the end against 64 bits."""
+    import torch
+
+    import gwenedeg_b200 as gw
+    c = gw.Context(0, n_attn=1, n_heads=8, n_kv_heads=2, head_dim=128, max_rows=rows)
+    gen = torch.Generator(device="cuda").manual_seed(n + rows)
+    lev = torch.randint(0, 256, (n, k // 2), generator=gen, dtype=torch.uint8, device="cuda")
+    sc = (torch.rand(n, k // gs, generator=gen, device="cuda") * 0.008 + 0.002).half()
+    xq = torch.randint(-127, 128, (rows, k), generator=gen, dtype=torch.int8, device="cuda")
+    xs = torch.rand(rows, k // gs, generator=gen, device="cuda") * 0.05 + 0.001
+    out = torch.empty(rows, n, device="cuda")
+    torch.cuda.synchronize()
+    w = c.q4_new_dev(n, k, gs, lev.data_ptr(), sc.data_ptr())
+    c.mm_q4_dev(w, rows, xq.data_ptr(), xs.data_ptr(), out.data_ptr())
+    c.sync()
+    rs = sorted({0, rows // 2, rows - 1})
+    fs = torch.cat([torch.arange(a, min(n, a + 40)) for a in (0, n // 2 - 7, n - 40)]).cuda()
+    levels = torch.stack((lev[fs] & 15, lev[fs] >> 4), 2).view(len(fs), k).to(torch.int8).cpu().numpy() - 8
+    want, tol = product(xq[rs].cpu().numpy(), xs[rs].cpu().numpy(), levels, sc[fs].cpu().numpy(), gs)
+    got = out[rs][:, fs].cpu().numpy()
+    assert (np.abs(got - want) <= tol).all()
+    w.free()
+    c.close()
+
+
 # ---- the plan of the products with many rows --------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
