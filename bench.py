@@ -509,6 +509,10 @@ def deltanet_leg(local_rank, steps, small=False, rank=0, world=1):
 def run_reference(args, rank, world):
     if rank != 0:
         return
+    from oracle import gwo
+    if gwo.load("ref") is None:  # (the restatement is this project's own code: its speed is not the reference's)
+        print(json.dumps({"impl": "reference", "unavailable": "the reference's sources were not there to build oracle/_ref from"}), flush=True)
+        return
     ctx_all = contexts()
     reps = max(1, args.steps)
     t0 = time.time()
