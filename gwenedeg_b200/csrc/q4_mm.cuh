@@ -112,6 +112,16 @@ __device__ __forceinline__ void mma_s8_first(int *d, const uint32_t *a, uint32_t
 constexpr int Q4_MAGIC = 0x4B400000;
 constexpr float Q4_MAGIC_F = 12582912.0f;
 
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
 // h = g sigmoid(g) u
 __device__ __forceinline__ float q4_silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
@@ -312,26 +322,19 @@ __global__ void __launch_bounds__(MOST, MOST > 256 ? 1 : NT == 1 && GS >= 64 ? 3
         if (a.hq) {
             // a group of GS outputs is spread over the GS / 16 CTAs of a cluster: they exchange their maxima
             constexpr int CL = GS / 16;
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            cluster_sync_all();
             for (int e = threadIdx.x; e < R * 16; e += blockDim.x) {
                 const int r = e >> 4, fo = e & 15;
                 float m = 0.0f;
 #pragma unroll
-                for (int q = 0; q < CL; q++) {
-                    uint32_t at;
-                    float v;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(top + r)), "r"(q));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
-                    m = fmaxf(m, v);
-                }
+                for (int q = 0; q < CL; q++) m = fmaxf(m, ld_cluster(top + r, q));
                 if (r < rows) {
                     const size_t f = (size_t)blockIdx.x * 16 + fo;
                     a.hq[(size_t)(row0 + r) * W.n + f] = wo_quant_level(h[e], quant_top(m));
                     if (f % GS == 0) a.hs[(size_t)(row0 + r) * (W.n / GS) + f / GS] = quant_scale(m);
                 }
             }
-            // (no CTA leaves while another may still read its maxima)
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            cluster_sync_all();  // (no CTA leaves while another may still read its maxima)
         }
     }
 }
@@ -421,16 +424,6 @@ __device__ __forceinline__ void ldg_stream8(const void *p, uint32_t *r) {
     asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "l"(p));
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
-    return v;
 }
 // Two adjacent rows of one output, as the halves of 64-bit registers (float2 values would be taken apart and put together again by moves)
 __device__ __forceinline__ uint64_t pack2(float x, float y) {

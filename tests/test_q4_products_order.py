@@ -403,6 +403,40 @@ def test_the_first_calls_of_a_process_in_several_threads():
         assert r.returncode == 0, r.stderr[-600:]
 
 
+# ---- waits that run out -----------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,gs", [(100, 264, 2176, 64), (300, 384, 8192, 128)])
+def test_an_expired_wait_is_reported_and_the_context_goes_on(ctx, dev, rows, n, k, gs):
+    """With the status word set by a wait that ran out the products give up their own waits early, but end; rq_cuda_sync reports it once."""
+    import gwenedeg_b200 as gw
+    rng = np.random.default_rng(k)
+    ms = [matrix(rng, n, k, gs) for _ in range(2)]
+    xq, xs = rows8(rng, rows, k, gs)
+    gate, up = (ctx.q4_new(packed(lev), sc, gs) for lev, sc in ms)
+    q, s, out = dev.put(xq), dev.put(xs * np.float32(0.1)), dev.room((rows, n), np.float32)
+    hq, hs = dev.room((rows, n // gs * gs), np.int8), dev.room((rows, n // gs), np.float32)
+
+    def calls():
+        ctx.mm_q4_dev(gate, rows, q, s, out)
+        if n % gs == 0:
+            ctx.ffn_q4_dev(gate, up, rows, q, s, None, hq, hs)
+
+    def results():
+        return dev.get(out, (rows, n)).view(np.uint32), dev.get(hq, (rows, n // gs * gs), np.int8), dev.get(hs, (rows, n // gs)).view(np.uint32)
+
+    calls()
+    want = results()
+    ctx.check(ctx.L.rq_cuda_selftest_wait_expiry(ctx.h, 1000))
+    calls()
+    with pytest.raises(gw.RqCudaError) as e:
+        ctx.sync()
+    assert e.value.code == -4 and "expired" in str(e.value)
+    ctx.sync()
+    calls()
+    for a, b in zip(results(), want):
+        assert np.array_equal(a, b)
+
+
 # ---- groups of very small values --------------------------------------------------------------------------------------
 SMALL = [2.0 ** e for e in (-100, -118, -119, -120, -121, -122, -124, -126, -130, -140)]
 LEAST = 2.0 ** -119  # what a group's largest magnitude counts as at least (rq_cuda.h)
