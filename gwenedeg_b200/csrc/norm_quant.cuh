@@ -13,7 +13,7 @@ namespace rq {
 // One CTA per row, thread t holds the float4s t, t + T, ... of the row in registers (V of them): x and d are read once, x', the
 // levels, the scales and y written once.  T and V depend on the row's width only, so a row's sum has one order whatever the
 // number of rows.  A group is 8, 16 or 32 adjacent lanes.  Sums in fp32: per thread, then a warp tree, then the warps in order.
-// Bound by the rows' bytes: 2048 x 4096 (x, d read, x', levels written) 19.2 us = 5.7 TB/s, 4096 x 8192 71 us = 6.2 TB/s; a single row
+// Bound by the rows' bytes: 2048 x 4096 (x, d read, x', levels written) 19.0 us = 5.8 TB/s, 4096 x 8192 70 us = 6.2 TB/s; a single row
 // of 4096 takes 2.4 us, the latency of a launch, one load and two reductions.
 struct NormQuantArgs {
     const float *x, *delta, *w;

@@ -138,7 +138,7 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src, bool valid
 // levels and scales (cp.async into the warp's own part of shared memory, rows 544 bytes apart: conflict-free 8-byte reads).  Outputs are M
 // of the MMA, rows N.  The slices' partial sums meet in shared memory and are added in order by the threads that own the outputs.
 // Bound by the weights' bytes; the weights' loads do not wait for the kernel before this one (they are constant), so they overlap its end.
-// Measured: 65536 x 4096 (groups of 64), one row, 24.9 us = 5.7 TB/s; walking over tiles with resident CTAs instead of one CTA per tile took
+// Measured: 65536 x 4096 (groups of 64), one row, 25.5 us = 5.6 TB/s; walking over tiles with resident CTAs instead of one CTA per tile took
 // 47 us, prefetching a later CTA's weights into the L2 cache 31 us.
 constexpr int Q4R_XROW = Q4_SLICE + 32;  // bytes from row to row of a slice's levels
 __host__ __device__ constexpr int q4r_warp_bytes(int gs, int nt) { return 8 * nt * (Q4R_XROW + Q4_SLICE / gs * 4); }
@@ -386,10 +386,12 @@ cudaError_t launch_q4_rows(const Q4Args &a, cudaStream_t stream) {
 //                   int8 rows of 128 inputs with the 128-byte swizzle (K-major A operand); the warp of a chunk's first quarter also asks
 //                   for the rows' levels by TMA (K-major B operand)
 //   one warp        issues the MMAs into two D buffers in turn, of as many groups as fill 128 columns (up to a chunk's)
-// What bounds it is the drain: per D value one logic operation, two multiply-adds and its part of the loads, about 1,900 warp instructions per
-// 128 x 128 group, of which 512 are packed multiply-adds on a pipe that takes one every two clocks, and two drain warps per scheduler that
-// issue half of the time: 960 clocks per group, against 128 for its products (tensor pipe 10 % busy, 16 % with groups of 128).  Measured:
-// 2000 x 6144 x 4096 268 us with groups of 64, 512 x 4096 x 12288 81 us with groups of 128 (633 TOP/s).  16 drain warps, TMEM loads ahead of their
+// What bounds it is the drain and what runs beside it.  Fitted over shapes, a chunk of 128 inputs of a 128 x 128 tile takes 650 clocks, whatever its
+// groups, and 960 per group, against 256 for its products (tensor pipe 10 % busy with groups of 64, 16 % with groups of 128).  A group's drain
+// is one logic operation and two multiply-adds per D value and its part of the loads, about 1,900 warp instructions, of which 512 are packed
+// multiply-adds on a pipe that takes one every two clocks; alone it takes 474 clocks.  The rest is not separated by a measurement: the unpack warps
+// on the same schedulers and the latencies of TMEM and shared memory, with two drain warps per scheduler and half of the issue slots empty.
+// Measured: 2000 x 6144 x 4096 270 us with groups of 64, 512 x 4096 x 12288 81.5 us with groups of 128 (632 TOP/s).  16 drain warps, TMEM loads ahead of their
 // use, and three buffers brought nothing; integer conversions instead of the offset cost 15 %, additions of the offset (which the compiler
 // puts on the multiply-add pipe) 5 %, three unpack warps instead of eight at 32 and 64 rows 40 %.
 // With few tiles the inputs are split over the C CTAs of a cluster at multiples of 1,024: every CTA leaves the sums of its pairs of slices
@@ -433,7 +435,7 @@ __device__ __forceinline__ uint64_t pack2(float x, float y) {
 }
 // p += round(16 D ws) xs for both rows, from the int32 sums d0, d1 (16 D); w2 = ws twice, o2 = -Q4_MAGIC_F w2.  The offset goes in by one
 // logic operation, (d & 0x7fffff) ^ 0x4B400000 (the sums fit 23 bits; flipping their sign bit adds 2^22): additions would be put on the pipe that
-// the multiply-adds need (630 against 530 clocks per 128 x 128 group in isolation).
+// the multiply-adds need (a sixth of the drain's time alone).
 __device__ __forceinline__ void q4_add2(uint64_t &p, uint32_t d0, uint32_t d1, uint64_t w2, uint64_t o2, uint64_t x2) {
     asm("{\n.reg .b32 a, b;\n.reg .b64 t;\nlop3.b32 a, %1, %6, %7, 0x6a;\nlop3.b32 b, %2, %6, %7, 0x6a;\nmov.b64 t, {a, b};\nfma.rn.f32x2 t, t, %3, %4;\nfma.rn.f32x2 %0, t, %5, %0;\n}"
         : "+l"(p)
@@ -839,8 +841,19 @@ cudaError_t launch_q4_tiles(const Q4Args &a, const Q4Plan &plan, Q4EncodeFn enc,
     return cudaLaunchKernelEx(&cfg, kern, a, map, plan.lst, plan.np, C, P, err);
 }
 
-// Up to this many rows the kernel for few rows is the faster one, in blocks of 8 or 16 rows (a block of 16 costs 1.75 blocks of 8).  Measured with
-// groups of 64: 48 x 6144 x 4096 14.3 against 20.3 us, 64 x 6144 x 4096 19.2 against 20.3 us, 64 x 4096 x 12288 38.3 against 30.5 us.
+// Up to this many rows the kernel for few rows runs, in blocks of 8 or 16 rows (a block of 16 is counted as 1.75 blocks of 8).  One number for all
+// shapes, right for most.  Measured, few rows / many rows in us:
+//   rows                           17            32            40            48            56            64
+//   6144 x 4096, groups of 32      11.0 / 18.6   13.0 / 18.7   17.5 / 28.6   17.6 / 28.6   21.9 / 28.6   23.7 / 28.7
+//   6144 x 4096, 64                 9.7 / 14.9   10.7 / 15.0   14.2 / 19.5   13.7 / 19.5   17.5 / 19.6   18.4 / 19.6
+//   4096 x 12288, 64               20.5 / 21.4   20.0 / 22.1   31.5 / 29.1   27.9 / 29.3   35.0 / 29.6   35.8 / 30.1
+//   4096 x 12288, 128              19.3 / 19.7   19.5 / 20.5   30.2 / 24.9   27.0 / 25.2   33.3 / 25.5   34.7 / 26.0
+//   65536 x 4096, 64               84.6 / 91.2   93.2 / 92.2    157 / 117     139 / 117     179 / 118     186 / 119
+//   gated 12288 x 4096, 64, 8-bit  42.0 / 47.5   45.8 / 47.8   67.3 / 63.5   66.1 / 63.5   83.5 / 63.6   84.9 / 63.7
+//   gated 12288 x 4096, 128        39.9 / 54.3   43.4 / 54.7   65.6 / 73.4   64.1 / 73.5   83.9 / 73.5   84.3 / 73.6
+// So it errs where the many-row kernel has enough tiles for the SMs or long inputs: from 33 rows on 65536 outputs (up to 1.5 x: the blocks of rows
+// also read such a matrix from memory once each), from 33 or 49 rows on 12288 inputs and on gated products with groups of 64 (up to 1.3 x).  40
+// rows (five blocks of 8) take up to 1.2 x of what 48 rows (three blocks of 16) take: a block of 16 costs less than 1.75 there.
 constexpr int Q4_FEW = 56;
 
 template <int GS>

@@ -33,7 +33,8 @@ struct Q4Plan {
 };
 // Rows per tile and CTAs along the inputs with the least estimated time, in clocks.  CTAs run one per SM, in waves; a CTA costs 6,000 to start
 // and end (2,500 more in a cluster) and a chunk of 128 inputs a part for its stage and a part per group that is drained, as measured:
-// 32 rows 750 + 190, 64 rows 700 + 500, 128 rows 650 + 960.
+// 32 rows 750 + 190, 64 rows 700 + 500, 128 rows 650 + 960.  Fitted to products: 2000 x 6144 x 4096 comes out as 269 us (measured 270), 512 x 4096 x
+// 12288 as 81.7 (81.5).  A gated product's epilogue is in no term: 1024 x 12288 x 4096 comes out as 494 us (measured 535).
 inline Q4Plan q4_plan(int rows, int w_tiles, int slices, int gs, bool gated, bool quant, int n_sm) {
     const int pairs = (slices + 1) / 2, tiles = (w_tiles + (gated ? 3 : 7)) / (gated ? 4 : 8), p = gated && quant && gs == 128 ? 2 : 1;
     Q4Plan best = {};

@@ -315,7 +315,9 @@ int rq_cuda_dn_out_dev(RqCuda *ctx, int lin_layer, const float *rows_dev, float 
  * decode layer is: rq_cuda_add_norm_quant_dev, rq_cuda_mm_q4_dev (q, k, v), rq_cuda_qk_norm_rope_store_dev, the attention
  * with rq_cuda_set_wo_quant, rq_cuda_mm_q4_dev (wo), rq_cuda_add_norm_quant_dev, rq_cuda_ffn_q4_dev, rq_cuda_mm_q4_dev (down).
  * These calls need no open pass; 1 <= rows <= max_rows.  They allocate nothing, use no scratch of the context and can be
- * captured into CUDA graphs.  Outputs must not overlap inputs except where a call says so.
+ * captured into CUDA graphs.  Outputs must not overlap inputs except where a call says so.  The calls return before their work is
+ * done.  A device-side wait that expires (0.2 s) leaves wrong numbers in the outputs, and only rq_cuda_sync says so: a host that waits for its
+ * own stream, or replays graphs, calls it before it relies on the results.
  *
  * A 4-bit weight matrix of n outputs x k inputs, laid out on the device once (RqCudaQ4).  levels: [n][k / 2] bytes, input 2 j
  * in the low half of byte j, input 2 j + 1 in the high half, each the level (-8 .. 7) + 8; scales: [n][k / gs] IEEE half bits;
@@ -330,18 +332,21 @@ size_t rq_cuda_q4_bytes(const RqCudaQ4 *w); /* device memory it holds */
  * inv = 1 / sqrt(mean(x'^2) + eps) and v = w x'; y = v inv (NULL: not written); xq, xs (both NULL: not written): per group of gs
  * values the levels of the library's quantiser (rq_cuda_set_wo_quant) on v and scale = max|v| (1 / 127) inv.  inv cancels out
  * of the levels: they are a function of x', w and the group alone.  A group's max|v| counts as at least 2^-119 (smaller ones have no
- * inverse in fp32), unless all of it is zero: then levels and scale are 0.  dim: a multiple of gs, at most 32768; gs 32, 64 or 128.
+ * inverse in fp32), unless all of it is zero: then levels and scale are 0.  The mean is taken in fp32: squares that overflow make inv
+ * 0.  A NaN in a row makes its y and its scales NaN.  dim: a multiple of gs, at most 32768; gs 32, 64 or 128.
  * x, x_out, delta, w, y 16-byte aligned; xq, xs 4-byte aligned. */
 int rq_cuda_add_norm_quant_dev(RqCuda *ctx, int rows, int dim, int gs, const float *x_dev, const float *delta_dev, const float *w_dev,
                                float eps, float *x_out_dev, float *y_dev, signed char *xq_dev, float *xs_dev);
 /* out[r][f] = sum over groups of xs[r][g] scale[f][g] (sum over the group of xq[r][k] level[f][k]): rows xq [rows][k], xs
  * [rows][k / gs] times the matrix, out fp32 [rows][n].  The inner sum is an exact integer; the outer one is in fp32 in one fixed
  * order (chains of fused multiply-adds inside slices of 512 inputs, slices added in pairs, pairs in order), so that a row's result does not
- * depend on the other rows of the call.  xq 16-byte aligned, xs and out 4-byte aligned. */
+ * depend on the other rows of the call.  The sums are carried as 16 times their value: from 2^124 on they become infinite.  xq 16-byte
+ * aligned, xs and out 4-byte aligned. */
 int rq_cuda_mm_q4_dev(RqCuda *ctx, const RqCudaQ4 *w, int rows, const signed char *xq_dev, const float *xs_dev, float *out_dev);
 /* The gated feed-forward product in one kernel: h = silu(x gate^T) (x up^T), silu(g) = g / (1 + e^-g), both products as
  * rq_cuda_mm_q4_dev.  h_dev: fp32 [rows][n]; hq_dev, hs_dev: the same rows through the library's quantiser, levels [rows][n] and
- * scales [rows][n / gs] with the matrices' gs (n a multiple of gs then; small groups as above), ready for the down product.  Either h_dev or the pair
+ * scales [rows][n / gs] with the matrices' gs (n a multiple of gs then; small groups as above; a NaN becomes level 0 and does not
+ * count for its group's scale, as in quantize()), ready for the down product.  Either h_dev or the pair
  * may be NULL.  gate and up have the same shape and gs; both may be the same matrix. */
 int rq_cuda_ffn_q4_dev(RqCuda *ctx, const RqCudaQ4 *gate, const RqCudaQ4 *up, int rows, const signed char *xq_dev, const float *xs_dev,
                        float *h_dev, signed char *hq_dev, float *hs_dev);
