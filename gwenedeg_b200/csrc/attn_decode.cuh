@@ -548,7 +548,7 @@ __device__ __forceinline__ int8_t wo_quant_level(float x, float wmax) {
 // soon 127 / m beyond fp32.  A level is then at most half of 2^-119 / 127 = 1.2e-38 off, the smallest normal number; a group of zeros has the scale 0.
 // (Multiplying small groups up instead keeps their relative precision, and cost the norm 2 to 8 %.)
 __device__ __forceinline__ float quant_top(float m) { return fmaxf(m, 0x1p-119f); }
-__device__ __forceinline__ float quant_scale(float m) { return m == 0.0f ? 0.0f : quant_top(m) * (1.0f / 127.0f); }
+__device__ __forceinline__ float quant_scale(float m) { return (m < 0x1p-119f && m != 0.0f ? 0x1p-119f : m) * (1.0f / 127.0f); }  // (NaN stays NaN)
 // where the merge kernels leave the quantised copy of their output rows: levels [rows][n_heads * head_dim] and one scale per
 // gs values (gs: 32, 64, 128 or 256, dividing head_dim); xq null: none
 struct WoQuant {

@@ -487,3 +487,14 @@ def test_gated_rows_quantise_groups_of_very_small_values(ctx, dev, rows, gs):
     assert (np.abs(lev - 127.0 * v / least[:, :, None]) <= 0.5 + 4 * 127 * 2.0 ** -24).all()
     want = np.where(top > 0, least / 127.0, 0.0)  # (the smallest rows may vanish)
     assert (np.abs(sc - want) <= 2 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.gpu
+def test_a_norm_weight_that_is_no_number_shows_in_the_scale(ctx, dev):
+    dim, gs = 256, 64
+    w = np.ones(dim, np.float32)
+    w[64:128] = np.nan
+    q, s = dev.room((2, dim), np.int8), dev.room((2, 4), np.float32)
+    ctx.add_norm_quant_dev(2, dim, gs, dev.put(np.ones((2, dim), np.float32)), None, dev.put(w), 1e-6, None, None, q, s)
+    sc = dev.get(s, (2, 4))
+    assert np.isnan(sc[:, 1]).all() and np.isfinite(sc[:, [0, 2, 3]]).all()
