@@ -173,11 +173,8 @@ static int fail(RqCuda *c, int code, const char *fmt, ...) {
                         cudaGetErrorString(e_));                                                             \
     } while (0)
 
-// ahead of the first launch of an attention or DeltaNet call
-static void behind_early(RqCuda *c) {
-    launch_in_order = c->early;
-    c->early = false;
-}
+// ahead of the first launch of an attention or DeltaNet call; c->early is cleared once that launch is made (a call may fail in between)
+static void behind_early(const RqCuda *c) { launch_in_order = c->early; }
 
 typedef CUresult (*TmEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1069,6 +1066,7 @@ static int launch_decode_with(RqCuda *c, int layer, const float *q, float *out, 
         default: e = cudaErrorInvalidValue;
     }
     if (e != cudaSuccess) return fail(c, RQ_CUDA_ERR_DEVICE, "attention launch: %s", cudaGetErrorString(e));
+    c->early = false;
     if (prof) cudaEventRecord(c->prof_ev[2 * c->prof_n++ + 1], c->stream);
     c->launches++;
     return launch_combine(c, q, out, part, ATT_P, 0);
@@ -1431,6 +1429,7 @@ static int launch_prefill(RqCuda *c, int layer, const float *q, float *out) {
         }
 #undef DEQUANT
         if (de != cudaSuccess) return fail(c, RQ_CUDA_ERR_DEVICE, "cache expansion launch: %s", cudaGetErrorString(de));
+        c->early = false;
         c->launches++;
         a.layer = 0;
         a.q = c->d_qrot;
@@ -1440,6 +1439,7 @@ static int launch_prefill(RqCuda *c, int layer, const float *q, float *out) {
     if (prof) cudaEventRecord(c->prof_ev[2 * c->prof_n], c->stream);
     cudaError_t e = hd == 128 ? launch_attn_prefill(a, c->stream) : launch_attn_prefill_hd256(a, c->stream);
     if (e != cudaSuccess) return fail(c, RQ_CUDA_ERR_DEVICE, "prefill attention launch: %s", cudaGetErrorString(e));
+    c->early = false;
     if (prof) cudaEventRecord(c->prof_ev[2 * c->prof_n++ + 1], c->stream);
     c->launches++;
     if (c->pf_quant) {
@@ -1705,6 +1705,7 @@ int rq_cuda_dn_chunk_dev(RqCuda *c, int lin_layer, const float *rows, float *out
     behind_early(c);
     cudaError_t e = launch_dn_chunk(a, c->stream);
     if (e != cudaSuccess) return fail(c, RQ_CUDA_ERR_DEVICE, "dn_chunk launch: %s", cudaGetErrorString(e));
+    c->early = false;
     c->launches += 2;
     return RQ_CUDA_OK;
 }

@@ -276,6 +276,10 @@ def test_attention_behind_a_product_waits_for_it_in_full():
         body = code[:code.index(launch)]
         body = body[body.rindex("\n}\n"):]  # the function's part in front of the launch
         assert "behind_early(c);" in body, launch
+        rest = code[code.index(launch):]
+        assert "c->early = false;" in rest[:rest.index("c->launches")], launch
+    helper = code[code.index("static void behind_early"):]
+    assert "early = " not in helper[:helper.index("}")].replace("in_order = c->early", "")  # (a call that fails before its launch leaves it to the next)
     for entry in ("rq_cuda_add_norm_quant_dev", "rq_cuda_mm_q4_dev", "rq_cuda_ffn_q4_dev"):
         body = code[code.index("int " + entry):]
         assert "c->early = true;" in body[:body.index("\n}\n")], entry
